@@ -440,6 +440,60 @@ int vil_optim_adamw_step_amp(const void* plan_dev, int nblocks, float beta1, flo
 int vil_optim_qhm_step_amp(const void* plan_dev, int nblocks, float momentum, float nu, int32_t* step_words,
                            const float* inv_scale, const float* found_inf, void* stream);
 
+/* ---- q and k between their projection and the attention: rotary positions with several axes (time, rows, columns), alone
+ * or behind the root-mean-square norm of every head (csrc/vil_qkrope.hip).  The reference's layers know positions only as
+ * relative_position_bias tables (src/models/layers/longformer2d.py:67-100); nothing of it is replaced here.
+ *
+ *   norm = 0:  y = R(theta) x                 norm = 1:  y = R(theta) (x w / sqrt(mean(x^2) + eps)),  per head row
+ *   theta_p = pos[b, n, axis(p)] * freq[p], p < R: the first sections[0] pairs turn with axis 0, the next with axis 1, ...
+ *   pair p = channels (p, R + p) [VIL_ROPE_HALF] or (2p, 2p + 1) [VIL_ROPE_INTERLEAVED]; channels >= 2R pass through
+ *
+ * q (B, N, Hq, M) and k (B, N, Hk, M) with the strides given (elements, channels contiguous): slices of a packed projection
+ * are read in place.  Hk = 0: no k.  R = 0 (norm only): pos, freq unused.  w (M), NULL = ones.  pos (B, N, axes), axes
+ * contiguous, pos_sb = 0 where all images share their positions.  Sums and statistics in fp32, angles in fp64.
+ * vil_qk_rope_bwd: gq / gk the gradients of yq / yk; dq / dk in q's dtype; dwq / dwk (M) in w_dtype, each NULL where it is not
+ * wanted, summed in a fixed order (workspace: vil_qk_rope_workspace_bytes; 0 bytes without norm); with norm = 0, q and k are
+ * not read (NULL). An output may not overlap an input. */
+enum { VIL_ROPE_HALF = 0, VIL_ROPE_INTERLEAVED = 1 };
+enum { VIL_POS_F32 = 0, VIL_POS_I32 = 1, VIL_POS_I64 = 2 };
+
+typedef struct VilRopeDesc {
+  int32_t B, N, Hq, Hk, M;        /* images, tokens, heads of q, heads of k (0: none), channels of a head (even, <= 256) */
+  int32_t R, axes, sections[4];   /* rotated pairs (2R <= M), position axes (<= 4), pairs of each axis (their sum is R)   */
+  int32_t layout;                 /* VIL_ROPE_*                                                                          */
+  int32_t dtype;                  /* VIL_DTYPE_F32 / _BF16 / _F16 of q, k, y, g, dq, dk                                   */
+  int32_t pos_dtype, freq_dtype;  /* VIL_POS_*; VIL_DTYPE_F32 / _F64                                                     */
+  int32_t norm, w_dtype;          /* w_dtype: VIL_DTYPE_F32 / _BF16 / _F16                                               */
+  float   eps;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh;          /* element strides (batch, token, head)                           */
+  int64_t yq_sb, yq_st, yq_sh, yk_sb, yk_st, yk_sh;    /* forward outputs                                                */
+  int64_t gq_sb, gq_st, gq_sh, gk_sb, gk_st, gk_sh;    /* backward: gradients of the outputs                             */
+  int64_t dq_sb, dq_st, dq_sh, dk_sb, dk_st, dk_sh;    /* backward: gradients of q, k                                    */
+  int64_t pos_sb, pos_st;
+} VilRopeDesc;
+
+size_t vil_qk_rope_workspace_bytes(const VilRopeDesc* d);
+int vil_qk_rope_fwd(const VilRopeDesc* d, const void* q, const void* k, const void* wq, const void* wk, const void* pos,
+                    const void* freq, void* yq, void* yk, void* stream);
+int vil_qk_rope_bwd(const VilRopeDesc* d, const void* gq, const void* gk, const void* q, const void* k, const void* wq,
+                    const void* wk, const void* pos, const void* freq, void* dq, void* dk, void* dwq, void* dwk,
+                    void* workspace, void* stream);
+
+/* ---- activations held in 8 bits between forward and backward (csrc/vil_act8.hip).  x (rows, cols) with a row stride, cols
+ * contiguous, fp32 / bf16 / fp16.  codes int8 (rows, cols), scales uint8 (rows, ceil(cols / 32)): 32 neighbouring channels of
+ * a row share 2^e, e = scale - 127 the smallest with max |x| <= 127 * 2^e (scale >= 1); code = round(x / 2^e), ties to
+ * even.  Scale 255: the block held an infinity or a NaN and comes back as NaN.
+ * vil_gelu_act8_fwd: a = gelu(h) (exact form) and the packed h.  vil_gelu_act8_bwd: with v = the values the packed h stands
+ * for, dh = da * gelu'(v) and, unless a is NULL, a = gelu(v): the input of the next projection's weight gradient, so that
+ * neither h nor gelu(h) need be kept in 16 bits (the reference keeps both: Mlp, src/models/msvit.py:17-34).
+ * a, dh and y are contiguous. */
+int vil_act8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t x_row_stride, void* codes, void* scales, void* stream);
+int vil_act8_unpack(const void* codes, const void* scales, int64_t rows, int cols, void* y, int dtype, void* stream);
+int vil_gelu_act8_fwd(const void* h, int dtype, int64_t rows, int cols, int64_t h_row_stride, void* a, void* codes, void* scales,
+                      void* stream);
+int vil_gelu_act8_bwd(const void* codes, const void* scales, const void* da, int dtype, int64_t rows, int cols,
+                      int64_t da_row_stride, void* dh, void* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,7 +40,9 @@ EXPORTS = ("vil_attn_abi_version", "vil_attn_strerror", "vil_attn_check", "vil_a
            "vil_resln_fwd", "vil_resln_bwd", "vil_gemm_workspace_bytes", "vil_gemm_bf16", "vil_gemm_tune", "vil_gemm_dgelu_bf16", "vil_gemm_gelu_bf16", "vil_gemm_tile_bf16", "vil_gemm_skinny_bf16", "vil_gemm_skinny_gelu_bf16",
            "vil_sc2d_qk", "vil_sc2d_av", "vil_sc2d_agrad", "vil_sc2d_mask",
            "vil_optim_plan_bytes", "vil_optim_plan_build", "vil_optim_adamw_step", "vil_optim_qhm_step",
-           "vil_optim_adamw_step_amp", "vil_optim_qhm_step_amp", "vil_attn_cw_set_shape", "vil_attn_cw_plan")
+           "vil_optim_adamw_step_amp", "vil_optim_qhm_step_amp", "vil_attn_cw_set_shape", "vil_attn_cw_plan",
+           "vil_qk_rope_workspace_bytes", "vil_qk_rope_fwd", "vil_qk_rope_bwd",
+           "vil_act8_pack", "vil_act8_unpack", "vil_gelu_act8_fwd", "vil_gelu_act8_bwd")
 
 
 class VilAttnDesc(ctypes.Structure):
@@ -53,6 +55,18 @@ class VilAttnDesc(ctypes.Structure):
 
 
 VIL_E_BACKEND = -10
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+POS_F32, POS_I32, POS_I64 = 0, 1, 2
+
+
+class VilRopeDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("B", "N", "Hq", "Hk", "M", "R", "axes")] +
+                [("sections", ctypes.c_int32 * 4)] +
+                [(n, ctypes.c_int32) for n in ("layout", "dtype", "pos_dtype", "freq_dtype", "norm", "w_dtype")] +
+                [("eps", ctypes.c_float)] +
+                [(t + s, ctypes.c_int64) for t in ("q", "k", "yq", "yk", "gq", "gk", "dq", "dk") for s in ("_sb", "_st", "_sh")] +
+                [("pos_sb", ctypes.c_int64), ("pos_st", ctypes.c_int64)])
 
 
 class VilOptimTensor(ctypes.Structure):
@@ -212,6 +226,22 @@ def lib():
         L.vil_patchify_fwd.argtypes = [vp, vp, ci, vp, vp, ci] + [ci] * 7 + [vp]
         L.vil_patchify_bwd.restype = ci
         L.vil_patchify_bwd.argtypes = [vp, ci, vp, vp, vp, ci] + [ci] * 7 + [vp]
+        if not (_AB_LIBRARY and not hasattr(L, "vil_qk_rope_fwd")):
+            rp = ctypes.POINTER(VilRopeDesc)
+            L.vil_qk_rope_workspace_bytes.restype = ctypes.c_size_t
+            L.vil_qk_rope_workspace_bytes.argtypes = [rp]
+            L.vil_qk_rope_fwd.restype = ci
+            L.vil_qk_rope_fwd.argtypes = [rp] + [vp] * 9
+            L.vil_qk_rope_bwd.restype = ci
+            L.vil_qk_rope_bwd.argtypes = [rp] + [vp] * 14
+            L.vil_act8_pack.restype = ci
+            L.vil_act8_pack.argtypes = [vp, ci, i64, ci, i64, vp, vp, vp]
+            L.vil_act8_unpack.restype = ci
+            L.vil_act8_unpack.argtypes = [vp, vp, i64, ci, vp, ci, vp]
+            L.vil_gelu_act8_fwd.restype = ci
+            L.vil_gelu_act8_fwd.argtypes = [vp, ci, i64, ci, i64, vp, vp, vp, vp]
+            L.vil_gelu_act8_bwd.restype = ci
+            L.vil_gelu_act8_bwd.argtypes = [vp, vp, vp, ci, i64, ci, i64, vp, vp, vp]
         if L.vil_attn_abi_version() != ABI_VERSION:
             raise RuntimeError("libvilattn.so ABI version mismatch; rebuild it")
         _lib = L

@@ -1,0 +1,303 @@
+// vil_qkrope.hip -- q and k of an attention layer between their projection and the attention: rotary positions with several
+// axes, alone or behind the root-mean-square norm of every head, forward and backward.
+//
+// Mathematics.  Pair p of a head (p < R) is rotated by theta = pos[axis(p)] * freq[p]:
+//     (u, v) -> (u cos - v sin, v cos + u sin)         u, v = channels p, R + p (VIL_ROPE_HALF) or 2p, 2p + 1 (INTERLEAVED)
+// channels from 2R on pass through.  With the norm, y = R(theta) (x r w), r = 1 / sqrt(mean x^2 + eps); its backward with
+// g = R(-theta) dy:   dw = sum over rows of g x r,   dx = r (g w - x r^2 mean(g w x)).  The mean, r and every sum are fp32;
+// a value is rounded once, where it is stored.
+//
+// Angles.  pos * freq / 2 pi is taken in fp64 and reduced to a quarter turn there, so that positions far into a stream keep
+// their angle (fp32 would lose 2^-24 of 10^5 radians: the whole fractional turn); sine and cosine of the remainder in
+// [-pi/4, pi/4] are their Taylor series in fp32 (next terms 2e-9 and 1e-10).
+#include "vil_internal.h"
+#include <string.h>
+
+namespace {
+
+constexpr int RO_AXES = 4;
+constexpr int RO_M_MAX = 256;
+constexpr int RO_THREADS = 256;
+
+struct RoSide {               // q or k
+  const void* x; const void* g; void* y; const void* w;
+  int64_t x_sb, x_st, x_sh, g_sb, g_st, g_sh, y_sb, y_st, y_sh;
+  int H;
+};
+struct RoParams {
+  RoSide s[2];
+  const void* pos; int64_t pos_sb, pos_st;
+  const void* freq;
+  float* parts;               // backward: (2, nblocks, M) partial sums of dw
+  int nblocks;                // workgroups of one side
+  int B, N, M, R, pos_dtype, freq_f64, w_dtype, interleaved;
+  int axes, sec_end[RO_AXES];
+  float eps, sign;            // sign: +1 rotates by theta, -1 back
+};
+
+// (the bf16 conversions of the compiler round to nearest even, v_cvt_pk_bf16_f32)
+template <typename T> __device__ __forceinline__ float ro_ld(const T* p) { return (float)*p; }
+template <typename T> __device__ __forceinline__ void ro_st(T* p, float v) { *p = (T)v; }
+
+__device__ __forceinline__ float ro_w(const void* w, int dtype, int i) {
+  if (!w) return 1.0f;
+  return dtype == VIL_DTYPE_F32 ? ((const float*)w)[i] : dtype == VIL_DTYPE_BF16 ? (float)((const __bf16*)w)[i] : (float)((const _Float16*)w)[i];
+}
+
+__device__ __forceinline__ void ro_sincos(const RoParams& p, int b, int n, int j, float& sn, float& cs) {
+  int axis = 0;
+  while (axis + 1 < p.axes && j >= p.sec_end[axis]) ++axis;
+  const int64_t at = b * p.pos_sb + n * p.pos_st + axis;
+  const double x = p.pos_dtype == VIL_POS_F32 ? (double)((const float*)p.pos)[at]
+                 : p.pos_dtype == VIL_POS_I32 ? (double)((const int32_t*)p.pos)[at] : (double)((const int64_t*)p.pos)[at];
+  const double f = p.freq_f64 ? ((const double*)p.freq)[j] : (double)((const float*)p.freq)[j];
+  double t = x * f * 0.15915494309189533577;           // turns
+  t = 4.0 * (t - floor(t));                            // quarter turns, [0, 4]
+  const double k = rint(t);
+  const float a = (float)(t - k) * 1.57079632679489662f, a2 = a * a;
+  float s0 = fmaf(a2, 2.7557319e-6f, -1.9841270e-4f), c0 = fmaf(a2, -2.7557319e-7f, 2.4801587e-5f);
+  s0 = fmaf(a2, s0, 8.3333333e-3f);  c0 = fmaf(a2, c0, -1.3888889e-3f);
+  s0 = fmaf(a2, s0, -1.6666667e-1f); c0 = fmaf(a2, c0, 4.1666667e-2f);
+  s0 = fmaf(a2 * a, s0, a);          c0 = fmaf(a2, c0, -0.5f);
+  c0 = fmaf(a2, c0, 1.0f);
+  const int q = (int)k;
+  const bool odd = q & 1;
+  const float s1 = odd ? c0 : s0, c1 = odd ? s0 : c0;
+  sn = (q & 2) ? -s1 : s1;
+  cs = ((q + 1) & 2) ? -c1 : c1;
+}
+
+template <int LPR>
+__device__ __forceinline__ float ro_row_sum(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Any even head of up to 256 channels, any strides: LPR lanes to a head row, NP pairs to a lane, one element at a time.
+// blockIdx.y: q or k.  BWD: y = dx, g = dy, x = the forward's input (read with NORM only).
+template <typename T, int LPR, int NP, bool NORM, bool BWD>
+__global__ __launch_bounds__(RO_THREADS) void k_rope_any(RoParams p) {
+  constexpr int RPW = 64 / LPR;
+  const RoSide& S = p.s[blockIdx.y];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPR, slot = lane / LPR;
+  const int64_t rows = (int64_t)p.B * p.N * S.H, per_pass = (int64_t)gridDim.x * 4 * RPW;
+  int c0[NP], c1[NP];
+  bool on[NP];
+  float w0[NP], w1[NP], d0[NP], d1[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int j = sub + i * LPR;
+    on[i] = j < p.M / 2;
+    const bool apart = j < p.R && !p.interleaved;
+    c0[i] = on[i] ? (apart ? j : 2 * j) : 0;
+    c1[i] = on[i] ? (apart ? p.R + j : 2 * j + 1) : 0;
+    w0[i] = NORM && on[i] ? ro_w(S.w, p.w_dtype, c0[i]) : 0.f;
+    w1[i] = NORM && on[i] ? ro_w(S.w, p.w_dtype, c1[i]) : 0.f;
+    d0[i] = d1[i] = 0.f;
+  }
+  for (int64_t r0 = ((int64_t)blockIdx.x * 4 + wave) * RPW; r0 < rows; r0 += per_pass) {
+    const int64_t row = r0 + slot;
+    const bool rok = row < rows;
+    const int64_t tok = row / S.H;
+    const int h = (int)(row - tok * S.H), b = (int)(tok / p.N), n = (int)(tok - (int64_t)b * p.N);
+    const T* x = (const T*)S.x + b * S.x_sb + n * S.x_st + h * S.x_sh;
+    const T* g = (const T*)S.g + b * S.g_sb + n * S.g_st + h * S.g_sh;
+    T* y = (T*)S.y + b * S.y_sb + n * S.y_st + h * S.y_sh;
+    float u[NP], v[NP], gu[NP], gv[NP], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const bool ok = rok && on[i];
+      const int j = sub + i * LPR;
+      u[i] = v[i] = gu[i] = gv[i] = 0.f;
+      if (ok) {
+        if (NORM || !BWD) { u[i] = ro_ld(x + c0[i]); v[i] = ro_ld(x + c1[i]); }
+        if (BWD) { gu[i] = ro_ld(g + c0[i]); gv[i] = ro_ld(g + c1[i]); }
+        if (BWD && j < p.R) {                       // g = R(-theta) dy
+          float sn, cs;
+          ro_sincos(p, b, n, j, sn, cs);
+          const float a = gu[i] * cs + gv[i] * sn;
+          gv[i] = gv[i] * cs - gu[i] * sn;
+          gu[i] = a;
+        }
+      }
+      if (NORM) { s1 = fmaf(u[i], u[i], s1); s1 = fmaf(v[i], v[i], s1); }
+      if (NORM && BWD) { s2 = fmaf(gu[i] * w0[i], u[i], s2); s2 = fmaf(gv[i] * w1[i], v[i], s2); }
+    }
+    float r = 1.f, m = 0.f;
+    if (NORM) {
+      r = 1.0f / sqrtf(ro_row_sum<LPR>(s1) / p.M + p.eps);
+      if (BWD) m = r * r * (ro_row_sum<LPR>(s2) / p.M);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int j = sub + i * LPR;
+      if (!(rok && on[i])) continue;
+      if (!BWD) {
+        float a = NORM ? u[i] * r * w0[i] : u[i], c = NORM ? v[i] * r * w1[i] : v[i];
+        if (j < p.R) {
+          float sn, cs;
+          ro_sincos(p, b, n, j, sn, cs);
+          const float a2 = a * cs - c * sn;
+          c = c * cs + a * sn;
+          a = a2;
+        }
+        ro_st(y + c0[i], a); ro_st(y + c1[i], c);
+      } else if (NORM) {
+        d0[i] = fmaf(gu[i], u[i] * r, d0[i]); d1[i] = fmaf(gv[i], v[i] * r, d1[i]);
+        ro_st(y + c0[i], r * (gu[i] * w0[i] - u[i] * m));
+        ro_st(y + c1[i], r * (gv[i] * w1[i] - v[i] * m));
+      } else {
+        ro_st(y + c0[i], gu[i]); ro_st(y + c1[i], gv[i]);
+      }
+    }
+  }
+  if (NORM && BWD && p.parts) {                       // rows of a wave, waves of a workgroup: one partial row of dw
+    __shared__ float red[4][RO_M_MAX];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+#pragma unroll
+      for (int o = LPR; o < 64; o <<= 1) { d0[i] += __shfl_xor(d0[i], o, 64); d1[i] += __shfl_xor(d1[i], o, 64); }
+      if (slot == 0 && on[i]) { red[wave][c0[i]] = d0[i]; red[wave][c1[i]] = d1[i]; }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.M; c += RO_THREADS)
+      p.parts[((int64_t)blockIdx.y * p.nblocks + blockIdx.x) * p.M + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  }
+}
+
+// dw of q and k from the workgroups' partial rows, in a fixed order.  One workgroup to 16 channels of a side; thread (i, c) adds the
+// rows i, i + 16, ... of its channel, the 16 sums of a channel are added in order.
+__global__ __launch_bounds__(256) void k_rope_dw(const float* parts, int nblocks, int M, void* dwq, void* dwk, int w_dtype) {
+  __shared__ float red[16][17];
+  void* dw = blockIdx.y ? dwk : dwq;
+  if (!dw) return;                                     // (uniform over the workgroup)
+  const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float s = 0.f;
+  if (c < M)
+    for (int i = sl; i < nblocks; i += 16) s += parts[((int64_t)blockIdx.y * nblocks + i) * M + c];
+  red[sl][cl] = s;
+  __syncthreads();
+  if (sl == 0 && c < M) {
+    for (int i = 1; i < 16; ++i) s += red[i][cl];
+    if (w_dtype == VIL_DTYPE_F32) ((float*)dw)[c] = s;
+    else if (w_dtype == VIL_DTYPE_BF16) ((__bf16*)dw)[c] = (__bf16)s;
+    else ((_Float16*)dw)[c] = (_Float16)s;
+  }
+}
+
+int ro_nblocks(const VilRopeDesc* d, int lpr) {
+  const int64_t rows = (int64_t)d->B * d->N * (d->Hq > d->Hk ? d->Hq : d->Hk);
+  const int64_t need = (rows + 4 * (64 / lpr) - 1) / (4 * (64 / lpr));
+  return (int)(need < 1024 ? (need < 1 ? 1 : need) : 1024);
+}
+
+int ro_lpr(int M) { return M <= 16 ? 8 : M <= 32 ? 16 : M <= 64 ? 32 : 64; }
+
+template <typename T, bool NORM, bool BWD>
+int ro_launch(const RoParams& p, int sides, hipStream_t s) {
+  const dim3 grid(p.nblocks, sides), block(RO_THREADS);
+  const int pairs = p.M / 2;
+  if (pairs <= 8) k_rope_any<T, 8, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
+  else if (pairs <= 16) k_rope_any<T, 16, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
+  else if (pairs <= 32) k_rope_any<T, 32, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
+  else if (pairs <= 64) k_rope_any<T, 64, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
+  else k_rope_any<T, 64, 2, NORM, BWD><<<grid, block, 0, s>>>(p);
+  return (int)hipGetLastError();
+}
+
+template <bool BWD>
+int ro_dispatch(const VilRopeDesc* d, const RoParams& p, hipStream_t s) {
+  const int sides = d->Hk > 0 ? 2 : 1;
+  switch (d->dtype * 2 + (d->norm ? 1 : 0)) {
+    case VIL_DTYPE_F32 * 2: return ro_launch<float, false, BWD>(p, sides, s);
+    case VIL_DTYPE_F32 * 2 + 1: return ro_launch<float, true, BWD>(p, sides, s);
+    case VIL_DTYPE_BF16 * 2: return ro_launch<__bf16, false, BWD>(p, sides, s);
+    case VIL_DTYPE_BF16 * 2 + 1: return ro_launch<__bf16, true, BWD>(p, sides, s);
+    case VIL_DTYPE_F16 * 2: return ro_launch<_Float16, false, BWD>(p, sides, s);
+    default: return ro_launch<_Float16, true, BWD>(p, sides, s);
+  }
+}
+
+int ro_check(const VilRopeDesc* d) {
+  if (!d) return VIL_E_NULL;
+  if (d->B < 0 || d->N < 0 || d->Hq <= 0 || d->Hk < 0) return VIL_E_SHAPE;
+  if ((int64_t)d->B * d->N > INT32_MAX) return VIL_E_SHAPE;
+  if (d->M < 2 || d->M % 2 || d->M > RO_M_MAX) return VIL_E_HEAD_DIM;
+  if (d->R < 0 || 2 * d->R > d->M || d->axes < 0 || d->axes > RO_AXES || (d->R > 0 && d->axes < 1)) return VIL_E_SHAPE;
+  int sum = 0;
+  for (int a = 0; a < d->axes; ++a) {
+    if (d->sections[a] < 0 || d->sections[a] > RO_M_MAX) return VIL_E_SHAPE;
+    sum += d->sections[a];
+  }
+  if (sum != d->R) return VIL_E_SHAPE;
+  if (d->layout != VIL_ROPE_HALF && d->layout != VIL_ROPE_INTERLEAVED) return VIL_E_MODE;
+  if (d->dtype != VIL_DTYPE_F32 && d->dtype != VIL_DTYPE_BF16 && d->dtype != VIL_DTYPE_F16) return VIL_E_DTYPE;
+  if (d->R > 0 && d->pos_dtype != VIL_POS_F32 && d->pos_dtype != VIL_POS_I32 && d->pos_dtype != VIL_POS_I64) return VIL_E_DTYPE;
+  if (d->R > 0 && d->freq_dtype != VIL_DTYPE_F32 && d->freq_dtype != VIL_DTYPE_F64) return VIL_E_DTYPE;
+  if (d->norm && d->w_dtype != VIL_DTYPE_F32 && d->w_dtype != VIL_DTYPE_BF16 && d->w_dtype != VIL_DTYPE_F16) return VIL_E_DTYPE;
+  if (!d->norm && d->R == 0) return VIL_E_SHAPE;          // nothing to do
+  return VIL_OK;
+}
+
+void ro_fill(RoParams& p, const VilRopeDesc* d, const void* pos, const void* freq) {
+  memset(&p, 0, sizeof(p));
+  p.B = d->B; p.N = d->N; p.M = d->M; p.R = d->R;
+  p.pos = pos; p.pos_sb = d->pos_sb; p.pos_st = d->pos_st; p.pos_dtype = d->pos_dtype;
+  p.freq = freq; p.freq_f64 = d->freq_dtype == VIL_DTYPE_F64;
+  p.w_dtype = d->w_dtype; p.interleaved = d->layout == VIL_ROPE_INTERLEAVED;
+  p.axes = d->axes;
+  for (int a = 0, e = 0; a < RO_AXES; ++a) p.sec_end[a] = e += a < d->axes ? d->sections[a] : 0;
+  p.eps = d->eps;
+  p.s[0].H = d->Hq; p.s[1].H = d->Hk;
+}
+#define RO_STRIDES(SIDE, F, NAME) SIDE.F##_sb = d->NAME##_sb, SIDE.F##_st = d->NAME##_st, SIDE.F##_sh = d->NAME##_sh
+
+}  // namespace
+
+extern "C" size_t vil_qk_rope_workspace_bytes(const VilRopeDesc* d) {
+  if (ro_check(d) || !d->norm) return 0;
+  return (size_t)2 * ro_nblocks(d, ro_lpr(d->M)) * d->M * sizeof(float);
+}
+
+extern "C" int vil_qk_rope_fwd(const VilRopeDesc* d, const void* q, const void* k, const void* wq, const void* wk,
+                               const void* pos, const void* freq, void* yq, void* yk, void* stream) {
+  if (int e = ro_check(d)) return e;
+  if (d->B == 0 || d->N == 0) return VIL_OK;
+  if (!q || !yq || (d->Hk > 0 && (!k || !yk)) || (d->R > 0 && (!pos || !freq))) return VIL_E_NULL;
+  RoParams p;
+  ro_fill(p, d, pos, freq);
+  p.s[0].x = q; p.s[0].y = yq; p.s[0].w = wq;
+  p.s[1].x = k; p.s[1].y = yk; p.s[1].w = wk;
+  RO_STRIDES(p.s[0], x, q); RO_STRIDES(p.s[0], y, yq);
+  RO_STRIDES(p.s[1], x, k); RO_STRIDES(p.s[1], y, yk);
+  p.nblocks = ro_nblocks(d, ro_lpr(d->M));
+  return ro_dispatch<false>(d, p, (hipStream_t)stream);
+}
+
+extern "C" int vil_qk_rope_bwd(const VilRopeDesc* d, const void* gq, const void* gk, const void* q, const void* k,
+                               const void* wq, const void* wk, const void* pos, const void* freq, void* dq, void* dk,
+                               void* dwq, void* dwk, void* workspace, void* stream) {
+  if (int e = ro_check(d)) return e;
+  const bool empty = d->B == 0 || d->N == 0;
+  if (!empty && (!gq || !dq || (d->Hk > 0 && (!gk || !dk)) || (d->R > 0 && (!pos || !freq)))) return VIL_E_NULL;
+  if (!empty && d->norm && (!q || (d->Hk > 0 && !k))) return VIL_E_NULL;
+  if ((dwq && (!d->norm || !wq)) || (dwk && (!d->norm || !wk || d->Hk == 0))) return VIL_E_NULL;
+  const bool dw = dwq || dwk;
+  if (dw && !workspace) return VIL_E_WORKSPACE;
+  RoParams p;
+  ro_fill(p, d, pos, freq);
+  p.s[0].g = gq; p.s[0].x = q; p.s[0].y = dq; p.s[0].w = wq;
+  p.s[1].g = gk; p.s[1].x = k; p.s[1].y = dk; p.s[1].w = wk;
+  RO_STRIDES(p.s[0], g, gq); RO_STRIDES(p.s[0], x, q); RO_STRIDES(p.s[0], y, dq);
+  RO_STRIDES(p.s[1], g, gk); RO_STRIDES(p.s[1], x, k); RO_STRIDES(p.s[1], y, dk);
+  p.parts = dw ? (float*)workspace : nullptr;
+  p.nblocks = empty ? 0 : ro_nblocks(d, ro_lpr(d->M));
+  if (!empty)
+    if (int e = ro_dispatch<true>(d, p, (hipStream_t)stream)) return e;
+  if (dw) {                                   // (an empty batch: zeros)
+    k_rope_dw<<<dim3((d->M + 15) / 16, 2), dim3(256), 0, (hipStream_t)stream>>>((const float*)workspace, p.nblocks, d->M, dwq, dwk, d->w_dtype);
+    return (int)hipGetLastError();
+  }
+  return VIL_OK;
+}
