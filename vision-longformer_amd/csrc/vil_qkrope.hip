@@ -33,6 +33,9 @@ struct RoParams {
   int B, N, M, R, pos_dtype, freq_f64, w_dtype, interleaved;
   int axes, sec_end[RO_AXES];
   float eps, sign;            // sign: +1 rotates by theta, -1 back
+  // tiled kernels: tokens of a tile (of all images in a row), tiles; magic numbers of x / H, x / N, x / R (0: divide)
+  int tile, ntiles;
+  unsigned h_magic[2], n_magic, r_magic;
 };
 
 // (the bf16 conversions of the compiler round to nearest even, v_cvt_pk_bf16_f32)
@@ -186,6 +189,342 @@ __global__ __launch_bounds__(256) void k_rope_dw(const float* parts, int nblocks
   }
 }
 
+// ---- tiled kernels: heads whose halves come in chunks of CH channels that a lane loads at once (16 bytes, or 8).
+// A lane owns CH pairs of a head row: two chunks, R apart (half) or side by side (interleaved, and channels that pass
+// through), so that a rotation needs no other lane and a row's statistics meet in LPR = M / (2 CH) neighbouring lanes
+// (rounded up to a power of two).  A workgroup takes a tile of tokens with all their heads: the angles of a token are taken once,
+// into LDS, while the first loads are under way, and serve every head.
+template <typename T, int CH> using ro_vec = T __attribute__((ext_vector_type(CH)));
+
+__device__ __forceinline__ unsigned ro_div(unsigned x, unsigned d, unsigned magic) { return magic ? __umulhi(x, magic) : x / d; }
+
+template <int CTRL> __device__ __forceinline__ float ro_dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// sum over LPR neighbouring lanes, in all of them (the mirrors pair lanes whose quads / eights already agree)
+template <int LPR> __device__ __forceinline__ float ro_lane_sum(float v) {
+  if (LPR >= 2) v += ro_dpp<0xb1>(v);           // quad_perm 1,0,3,2
+  if (LPR >= 4) v += ro_dpp<0x4e>(v);           // quad_perm 2,3,0,1
+  if (LPR >= 8) v += ro_dpp<0x141>(v);          // row_half_mirror
+  if (LPR >= 16) v += ro_dpp<0x140>(v);         // row_mirror
+  if (LPR >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+// where token tt of the tile that starts at token (b0, n0) lies
+__device__ __forceinline__ void ro_token(const RoParams& p, int b0, int n0, int tt, int& b, int& n) {
+  const unsigned x = (unsigned)(n0 + tt), q = ro_div(x, p.N, p.n_magic);
+  b = b0 + (int)q;
+  n = (int)(x - q * p.N);
+}
+
+// cosines and sines of a tile, trig[tt * R + j]
+__device__ __forceinline__ void ro_tile_angles(const RoParams& p, float2* trig, int b0, int n0, int ntok) {
+  for (int e = threadIdx.x; e < ntok * p.R; e += RO_THREADS) {
+    const int tt = (int)ro_div(e, p.R, p.r_magic), j = e - tt * p.R;
+    int b, n;
+    ro_token(p, b0, n0, tt, b, n);
+    float sn, cs;
+    ro_sincos(p, b, n, j, sn, cs);
+    trig[e] = make_float2(cs, sn);
+  }
+}
+
+// a lane's pairs: chunk a at channel ca, chunk b at cb; HALF pairs a[i] with b[i], INTERLEAVED neighbours
+struct RoUnit { int ca, cb, j0; bool on, turns; };
+template <int CH> __device__ __forceinline__ RoUnit ro_unit(const RoParams& p, int sub) {
+  RoUnit u;
+  u.on = sub * 2 * CH < p.M;
+  u.j0 = sub * CH;
+  u.turns = u.on && u.j0 < p.R;
+  const bool apart = u.turns && !p.interleaved;
+  u.ca = u.on ? (apart ? u.j0 : 2 * u.j0) : 0;
+  u.cb = u.on ? (apart ? p.R + u.j0 : 2 * u.j0 + CH) : CH;
+  return u;
+}
+
+template <int CH>
+__device__ __forceinline__ void ro_turn(float (&a)[CH], float (&b)[CH], const float2* cs, bool interleaved, float sign) {
+  if (!interleaved) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const float2 t = cs[i];
+      const float sn = t.y * sign, x = a[i] * t.x - b[i] * sn;
+      b[i] = b[i] * t.x + a[i] * sn;
+      a[i] = x;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; i += 2) {
+      const float2 t = cs[i / 2], v = cs[CH / 2 + i / 2];
+      const float ts = t.y * sign, vs = v.y * sign, x = a[i] * t.x - a[i + 1] * ts, y = b[i] * v.x - b[i + 1] * vs;
+      a[i + 1] = a[i + 1] * t.x + a[i] * ts;
+      a[i] = x;
+      b[i + 1] = b[i + 1] * v.x + b[i] * vs;
+      b[i] = y;
+    }
+  }
+}
+
+// The forward pass; without the norm the backward pass too (sign -1).
+template <typename T, int CH, int LPR, bool NORM>
+__global__ __launch_bounds__(RO_THREADS) void k_rope_tile(RoParams p) {
+  constexpr int ROWS = RO_THREADS / LPR, IPT = 4;
+  extern __shared__ float ro_lds[];
+  float* wl = ro_lds;                                            // (2, M) weights of q, k
+  float2* trig = (float2*)(ro_lds + (NORM ? 2 * p.M : 0));
+  const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+  const int64_t t0 = (int64_t)blockIdx.x * p.tile;
+  const int b0 = (int)(t0 / p.N), n0 = (int)(t0 - (int64_t)b0 * p.N);
+  const int64_t left = (int64_t)p.B * p.N - t0;
+  const int ntok = left < p.tile ? (int)left : p.tile, HH = p.s[0].H + p.s[1].H, items = ntok * HH;
+  const RoUnit u = ro_unit<CH>(p, sub);
+  bool first = true;
+  for (int base = 0; base < items; base += IPT * ROWS) {
+    ro_vec<T, CH> xa[IPT], xb[IPT];
+    int tok[IPT];
+    T* y[IPT];
+    bool ok[IPT], key[IPT];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int idx = base + i * ROWS + slot;
+      ok[i] = idx < items && u.on;
+      const int tt = (int)ro_div(idx, HH, p.h_magic[0]), h = idx - tt * HH;
+      key[i] = h >= p.s[0].H;
+      const RoSide& S = p.s[key[i] ? 1 : 0];
+      int b, n;
+      ro_token(p, b0, n0, tt, b, n);
+      tok[i] = tt;
+      const int hs = key[i] ? h - p.s[0].H : h;
+      y[i] = (T*)S.y + b * S.y_sb + n * S.y_st + hs * S.y_sh;
+      if (ok[i]) {
+        const T* x = (const T*)S.x + b * S.x_sb + n * S.x_st + hs * S.x_sh;
+        xa[i] = *(const ro_vec<T, CH>*)(x + u.ca);
+        xb[i] = *(const ro_vec<T, CH>*)(x + u.cb);
+      }
+    }
+    if (first) {
+      first = false;
+      if (NORM)
+        for (int c = threadIdx.x; c < 2 * p.M; c += RO_THREADS) wl[c] = c < p.M ? ro_w(p.s[0].w, p.w_dtype, c) : ro_w(p.s[1].w, p.w_dtype, c - p.M);
+      ro_tile_angles(p, trig, b0, n0, ntok);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      float a[CH], b[CH], r = 1.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) { a[c] = ok[i] ? (float)xa[i][c] : 0.f; b[c] = ok[i] ? (float)xb[i][c] : 0.f; }
+      if (NORM) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) { s = fmaf(a[c], a[c], s); s = fmaf(b[c], b[c], s); }
+        r = 1.0f / sqrtf(ro_lane_sum<LPR>(s) / p.M + p.eps);
+      }
+      if (!ok[i]) continue;
+      if (NORM) {
+        const float* w = wl + (key[i] ? p.M : 0);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) { a[c] = a[c] * r * w[u.ca + c]; b[c] = b[c] * r * w[u.cb + c]; }
+      }
+      if (u.turns) ro_turn<CH>(a, b, trig + tok[i] * p.R + u.j0, p.interleaved, p.sign);
+      ro_vec<T, CH> oa, ob;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) { oa[c] = (T)a[c]; ob[c] = (T)b[c]; }
+      *(ro_vec<T, CH>*)(y[i] + u.ca) = oa;
+      *(ro_vec<T, CH>*)(y[i] + u.cb) = ob;
+    }
+  }
+}
+
+// The norm's backward pass.  blockIdx.y: q or k; a workgroup walks tiles and keeps its share of dw in registers.
+template <typename T, int CH, int LPR>
+__global__ __launch_bounds__(RO_THREADS) void k_rope_norm_bwd(RoParams p) {
+  constexpr int ROWS = RO_THREADS / LPR, IPT = 2;
+  extern __shared__ float ro_lds[];
+  float2* trig = (float2*)ro_lds;
+  __shared__ float red[4][RO_M_MAX];
+  const RoSide& S = p.s[blockIdx.y];
+  const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR, wave = threadIdx.x >> 6;
+  const RoUnit u = ro_unit<CH>(p, sub);
+  float wa[CH], wb[CH], da[CH], db[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    wa[c] = ro_w(S.w, p.w_dtype, u.ca + c);
+    wb[c] = ro_w(S.w, p.w_dtype, u.cb + c);
+    da[c] = db[c] = 0.f;
+  }
+  for (int tile = blockIdx.x; tile < p.ntiles; tile += gridDim.x) {
+    const int64_t t0 = (int64_t)tile * p.tile;
+    const int b0 = (int)(t0 / p.N), n0 = (int)(t0 - (int64_t)b0 * p.N);
+    const int64_t left = (int64_t)p.B * p.N - t0;
+    const int ntok = left < p.tile ? (int)left : p.tile, items = ntok * S.H;
+    bool first = true;
+    for (int base = 0; base < items; base += IPT * ROWS) {
+      ro_vec<T, CH> xa[IPT], xb[IPT], ya[IPT], yb[IPT];
+      T* o[IPT];
+      int tok[IPT];
+      bool ok[IPT];
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        const int idx = base + i * ROWS + slot;
+        ok[i] = idx < items && u.on;
+        const int tt = (int)ro_div(idx, S.H, p.h_magic[blockIdx.y]), h = idx - tt * S.H;
+        int b, n;
+        ro_token(p, b0, n0, tt, b, n);
+        tok[i] = tt;
+        o[i] = (T*)S.y + b * S.y_sb + n * S.y_st + h * S.y_sh;
+        if (ok[i]) {
+          const T* x = (const T*)S.x + b * S.x_sb + n * S.x_st + h * S.x_sh;
+          const T* g = (const T*)S.g + b * S.g_sb + n * S.g_st + h * S.g_sh;
+          xa[i] = *(const ro_vec<T, CH>*)(x + u.ca);
+          xb[i] = *(const ro_vec<T, CH>*)(x + u.cb);
+          ya[i] = *(const ro_vec<T, CH>*)(g + u.ca);
+          yb[i] = *(const ro_vec<T, CH>*)(g + u.cb);
+        }
+      }
+      if (first) {
+        first = false;
+        ro_tile_angles(p, trig, b0, n0, ntok);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        float a[CH], b[CH], ga[CH], gb[CH], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          a[c] = ok[i] ? (float)xa[i][c] : 0.f; b[c] = ok[i] ? (float)xb[i][c] : 0.f;
+          ga[c] = ok[i] ? (float)ya[i][c] : 0.f; gb[c] = ok[i] ? (float)yb[i][c] : 0.f;
+        }
+        if (u.turns && ok[i]) ro_turn<CH>(ga, gb, trig + tok[i] * p.R + u.j0, p.interleaved, -1.0f);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          s1 = fmaf(a[c], a[c], s1); s1 = fmaf(b[c], b[c], s1);
+          s2 = fmaf(ga[c] * wa[c], a[c], s2); s2 = fmaf(gb[c] * wb[c], b[c], s2);
+        }
+        const float r = 1.0f / sqrtf(ro_lane_sum<LPR>(s1) / p.M + p.eps), m = r * r * (ro_lane_sum<LPR>(s2) / p.M);
+        if (!ok[i]) continue;
+        ro_vec<T, CH> oa, ob;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          da[c] = fmaf(ga[c], a[c] * r, da[c]);
+          db[c] = fmaf(gb[c], b[c] * r, db[c]);
+          oa[c] = (T)(r * (ga[c] * wa[c] - a[c] * m));
+          ob[c] = (T)(r * (gb[c] * wb[c] - b[c] * m));
+        }
+        *(ro_vec<T, CH>*)(o[i] + u.ca) = oa;
+        *(ro_vec<T, CH>*)(o[i] + u.cb) = ob;
+      }
+    }
+    __syncthreads();                                   // the next tile's angles overwrite this one's
+  }
+  if (!p.parts) return;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int k = LPR; k < 64; k <<= 1) { da[c] += __shfl_xor(da[c], k, 64); db[c] += __shfl_xor(db[c], k, 64); }
+    if ((threadIdx.x & 63) < LPR && u.on) { red[wave][u.ca + c] = da[c]; red[wave][u.cb + c] = db[c]; }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.M; c += RO_THREADS)
+    p.parts[((int64_t)blockIdx.y * p.nblocks + blockIdx.x) * p.M + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+
+unsigned ro_magic(int64_t most, int64_t d) {           // x / d == umulhi(x, magic) for every x <= most, else 0
+  const uint64_t m = ((1ull << 32) + (uint64_t)d - 1) / (uint64_t)d;
+  if (d < 2 || m >= (1ull << 32) || most >= (1ll << 32)) return 0;
+  return (m * (uint64_t)d - (1ull << 32)) * (uint64_t)most < (1ull << 32) ? (unsigned)m : 0u;
+}
+
+// Channels of a chunk: 16 bytes where the head, the rotated part and every stride and address allow it, else 8 bytes of a 16-bit
+// type, else 0: one element at a time.
+int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
+  const int size = dtype == VIL_DTYPE_F32 ? 4 : 2;
+  for (int ch = 16 / size; ch >= 4; ch /= 2) {
+    if (p.M % (2 * ch) || p.R % ch) continue;
+    uintptr_t bits = 0;
+    for (int i = 0; i < 2; ++i) {
+      const RoSide& S = p.s[i];
+      if (!S.H) continue;
+      bits |= (uintptr_t)S.x | (uintptr_t)S.y | (uintptr_t)(S.x_sb | S.x_st | S.x_sh | S.y_sb | S.y_st | S.y_sh) * size;
+      if (bwd_norm) bits |= (uintptr_t)S.g | (uintptr_t)(S.g_sb | S.g_st | S.g_sh) * size;
+    }
+    if (bits % (ch * size) == 0) return ch;
+  }
+  return 0;
+}
+
+// tokens of a tile: `ipt` head rows to a thread, angles in 16 KB, and no larger than leaves `want` tiles
+int ro_tile(const RoParams& p, int lpr, int heads, int ipt, int64_t want) {
+  const int64_t tokens = (int64_t)p.B * p.N;
+  int64_t t = (int64_t)ipt * (RO_THREADS / lpr) / heads;
+  if (p.R > 0 && t > 2048 / p.R) t = 2048 / p.R;
+  if (t > (tokens + want - 1) / want) t = (tokens + want - 1) / want;
+  return t < 1 ? 1 : (int)t;
+}
+
+template <typename T, int CH, int LPR, bool NORM>
+int ro_tile_launch(RoParams& p, hipStream_t s) {
+  const int HH = p.s[0].H + p.s[1].H;
+  p.tile = ro_tile(p, LPR, HH, 4, 1024);
+  p.h_magic[0] = ro_magic((int64_t)p.tile * HH + 4 * RO_THREADS, HH);
+  p.n_magic = ro_magic((int64_t)p.N + p.tile + 4 * RO_THREADS, p.N);
+  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
+  const int64_t tiles = ((int64_t)p.B * p.N + p.tile - 1) / p.tile;
+  const size_t lds = (NORM ? 2 * p.M * sizeof(float) : 0) + (size_t)p.tile * p.R * sizeof(float2);
+  k_rope_tile<T, CH, LPR, NORM><<<dim3((unsigned)tiles), dim3(RO_THREADS), lds, s>>>(p);
+  return (int)hipGetLastError();
+}
+
+constexpr int RO_BWD_BLOCKS = 1024;                    // workgroups of one side at the most: rows of partial sums
+
+template <typename T, int CH, int LPR>
+int ro_bwd_launch(RoParams& p, int sides, hipStream_t s) {
+  const int H = p.s[0].H > p.s[1].H ? p.s[0].H : p.s[1].H;
+  p.tile = ro_tile(p, LPR, H, 2, 1024);
+  for (int i = 0; i < sides; ++i) p.h_magic[i] = ro_magic((int64_t)p.tile * p.s[i].H + 2 * RO_THREADS, p.s[i].H);
+  p.n_magic = ro_magic((int64_t)p.N + p.tile + 2 * RO_THREADS, p.N);
+  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
+  p.ntiles = (int)(((int64_t)p.B * p.N + p.tile - 1) / p.tile);
+  p.nblocks = p.ntiles < RO_BWD_BLOCKS ? p.ntiles : RO_BWD_BLOCKS;
+  k_rope_norm_bwd<T, CH, LPR><<<dim3(p.nblocks, sides), dim3(RO_THREADS), (size_t)p.tile * p.R * sizeof(float2), s>>>(p);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int CH, bool NORM>
+int ro_tile_lanes(RoParams& p, hipStream_t s) {
+  const int lanes = p.M / (2 * CH);
+  if (lanes <= 1) return ro_tile_launch<T, CH, 1, NORM>(p, s);
+  if (lanes <= 2) return ro_tile_launch<T, CH, 2, NORM>(p, s);
+  if (lanes <= 4) return ro_tile_launch<T, CH, 4, NORM>(p, s);
+  if (lanes <= 8) return ro_tile_launch<T, CH, 8, NORM>(p, s);
+  if (lanes <= 16) return ro_tile_launch<T, CH, 16, NORM>(p, s);
+  return ro_tile_launch<T, CH, 32, NORM>(p, s);
+}
+template <typename T, int CH>
+int ro_bwd_lanes(RoParams& p, int sides, hipStream_t s) {
+  const int lanes = p.M / (2 * CH);
+  if (lanes <= 1) return ro_bwd_launch<T, CH, 1>(p, sides, s);
+  if (lanes <= 2) return ro_bwd_launch<T, CH, 2>(p, sides, s);
+  if (lanes <= 4) return ro_bwd_launch<T, CH, 4>(p, sides, s);
+  if (lanes <= 8) return ro_bwd_launch<T, CH, 8>(p, sides, s);
+  if (lanes <= 16) return ro_bwd_launch<T, CH, 16>(p, sides, s);
+  return ro_bwd_launch<T, CH, 32>(p, sides, s);
+}
+template <typename T, bool NORM, bool BWD>
+int ro_tiled(RoParams& p, int ch, int sides, hipStream_t s) {
+  if constexpr (NORM && BWD) {
+    if constexpr (sizeof(T) == 2)
+      if (ch == 8) return ro_bwd_lanes<T, 8>(p, sides, s);
+    return ro_bwd_lanes<T, 4>(p, sides, s);
+  } else {
+    p.sign = BWD ? -1.0f : 1.0f;
+    if constexpr (sizeof(T) == 2)
+      if (ch == 8) return ro_tile_lanes<T, 8, NORM>(p, s);
+    return ro_tile_lanes<T, 4, NORM>(p, s);
+  }
+}
+
 int ro_nblocks(const VilRopeDesc* d, int lpr) {
   const int64_t rows = (int64_t)d->B * d->N * (d->Hq > d->Hk ? d->Hq : d->Hk);
   const int64_t need = (rows + 4 * (64 / lpr) - 1) / (4 * (64 / lpr));
@@ -195,7 +534,11 @@ int ro_nblocks(const VilRopeDesc* d, int lpr) {
 int ro_lpr(int M) { return M <= 16 ? 8 : M <= 32 ? 16 : M <= 64 ? 32 : 64; }
 
 template <typename T, bool NORM, bool BWD>
-int ro_launch(const RoParams& p, int sides, hipStream_t s) {
+int ro_launch(RoParams& p, int dtype, int sides, hipStream_t s) {
+  // (without the norm the backward pass reads g alone)
+  if (BWD && !NORM)
+    for (int i = 0; i < 2; ++i) { p.s[i].x = p.s[i].g; p.s[i].x_sb = p.s[i].g_sb; p.s[i].x_st = p.s[i].g_st; p.s[i].x_sh = p.s[i].g_sh; }
+  if (const int ch = ro_chunk(p, dtype, NORM && BWD)) return ro_tiled<T, NORM, BWD>(p, ch, sides, s);
   const dim3 grid(p.nblocks, sides), block(RO_THREADS);
   const int pairs = p.M / 2;
   if (pairs <= 8) k_rope_any<T, 8, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
@@ -207,15 +550,15 @@ int ro_launch(const RoParams& p, int sides, hipStream_t s) {
 }
 
 template <bool BWD>
-int ro_dispatch(const VilRopeDesc* d, const RoParams& p, hipStream_t s) {
+int ro_dispatch(const VilRopeDesc* d, RoParams& p, hipStream_t s) {
   const int sides = d->Hk > 0 ? 2 : 1;
   switch (d->dtype * 2 + (d->norm ? 1 : 0)) {
-    case VIL_DTYPE_F32 * 2: return ro_launch<float, false, BWD>(p, sides, s);
-    case VIL_DTYPE_F32 * 2 + 1: return ro_launch<float, true, BWD>(p, sides, s);
-    case VIL_DTYPE_BF16 * 2: return ro_launch<__bf16, false, BWD>(p, sides, s);
-    case VIL_DTYPE_BF16 * 2 + 1: return ro_launch<__bf16, true, BWD>(p, sides, s);
-    case VIL_DTYPE_F16 * 2: return ro_launch<_Float16, false, BWD>(p, sides, s);
-    default: return ro_launch<_Float16, true, BWD>(p, sides, s);
+    case VIL_DTYPE_F32 * 2: return ro_launch<float, false, BWD>(p, d->dtype, sides, s);
+    case VIL_DTYPE_F32 * 2 + 1: return ro_launch<float, true, BWD>(p, d->dtype, sides, s);
+    case VIL_DTYPE_BF16 * 2: return ro_launch<__bf16, false, BWD>(p, d->dtype, sides, s);
+    case VIL_DTYPE_BF16 * 2 + 1: return ro_launch<__bf16, true, BWD>(p, d->dtype, sides, s);
+    case VIL_DTYPE_F16 * 2: return ro_launch<_Float16, false, BWD>(p, d->dtype, sides, s);
+    default: return ro_launch<_Float16, true, BWD>(p, d->dtype, sides, s);
   }
 }
 
@@ -257,7 +600,10 @@ void ro_fill(RoParams& p, const VilRopeDesc* d, const void* pos, const void* fre
 
 extern "C" size_t vil_qk_rope_workspace_bytes(const VilRopeDesc* d) {
   if (ro_check(d) || !d->norm) return 0;
-  return (size_t)2 * ro_nblocks(d, ro_lpr(d->M)) * d->M * sizeof(float);
+  // a row of partial sums to a workgroup of either kernel: the tiled one has at most one to a token
+  const int64_t tokens = (int64_t)d->B * d->N, tiled = tokens < RO_BWD_BLOCKS ? tokens : RO_BWD_BLOCKS;
+  const int64_t any = ro_nblocks(d, ro_lpr(d->M));
+  return (size_t)2 * (tiled > any ? tiled : any) * d->M * sizeof(float);
 }
 
 extern "C" int vil_qk_rope_fwd(const VilRopeDesc* d, const void* q, const void* k, const void* wq, const void* wk,
