@@ -198,13 +198,24 @@ def test_strides_and_alignment(how):
     want = rotary.vil_qk_norm_rope(qc, kc, wq, wq, **{**kw, "positions": pos.contiguous()})
     q, k = q.detach().requires_grad_(), k.detach().requires_grad_()
     got = rotary.vil_qk_norm_rope(q, k, wq, wq, **kw)
+
+    def same(a, b):
+        # A layout that the 16-byte loads do not fit adds a row's M squares and products in another order: r and the mean differ by
+        # up to 2 (M + 8) u relative, so a value moves by that share of its pair's and its row's scale (at most 4 (|a| + |b|) of
+        # these inputs' largest) and may round to the neighbouring number: one step of the type, eps |b|, or its smallest one.
+        if how in ("heads_first", "expanded_batch"):
+            return torch.equal(a, b)
+        a, b = a.double(), b.double()
+        f = torch.finfo(t)
+        return bool(((a - b).abs() <= f.eps * b.abs() * (1 + f.eps) + f.tiny * f.eps + 2 * (M + 8) * U * 4 * b.abs().amax()).all())
+
     for a, b in zip(got, want):
-        assert torch.equal(a, b) and a.is_contiguous()
+        assert same(a, b) and a.is_contiguous()
     # a gradient that is a slice, and one that is a single broadcast number
     gq = n(B, N, H, 2 * M)[..., M:]
     gk = torch.ones((), device="cuda", dtype=t).expand(B, N, H, M)
     for a, b in zip(torch.autograd.grad(got, (q, k), (gq, gk)), torch.autograd.grad(want, (qc, kc), (gq.contiguous(), gk.contiguous()))):
-        assert torch.equal(a, b)
+        assert same(a, b)
 
 
 @pytest.mark.parametrize("shape", [(0, 5), (3, 0)])

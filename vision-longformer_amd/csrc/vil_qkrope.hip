@@ -33,9 +33,12 @@ struct RoParams {
   int B, N, M, R, pos_dtype, freq_f64, w_dtype, interleaved;
   int axes, sec_end[RO_AXES];
   float eps, sign;            // sign: +1 rotates by theta, -1 back
-  // tiled kernels: tokens of a tile (of all images in a row), tiles; magic numbers of x / H, x / N, x / R (0: divide)
-  int tile, ntiles;
+  // tiled kernels: tokens of a tile, tiles of a segment, segments, segments of a workgroup, tokens of a segment; magic numbers of
+  // x / H, x / N, x / R (0: divide)
+  int sides, tile, ntiles, nseg, spg, flat, shared;
+  int64_t T;
   unsigned h_magic[2], n_magic, r_magic;
+  float inv_m;
 };
 
 // (the bf16 conversions of the compiler round to nearest even, v_cvt_pk_bf16_f32)
@@ -129,8 +132,8 @@ __global__ __launch_bounds__(RO_THREADS) void k_rope_any(RoParams p) {
     }
     float r = 1.f, m = 0.f;
     if (NORM) {
-      r = 1.0f / sqrtf(ro_row_sum<LPR>(s1) / p.M + p.eps);
-      if (BWD) m = r * r * (ro_row_sum<LPR>(s2) / p.M);
+      r = __builtin_amdgcn_rsqf(fmaf(ro_row_sum<LPR>(s1), p.inv_m, p.eps));
+      if (BWD) m = r * r * (ro_row_sum<LPR>(s2) * p.inv_m);
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -170,30 +173,50 @@ __global__ __launch_bounds__(RO_THREADS) void k_rope_any(RoParams p) {
 }
 
 // dw of q and k from the workgroups' partial rows, in a fixed order.  One workgroup to 16 channels of a side; thread (i, c) adds the
-// rows i, i + 16, ... of its channel, the 16 sums of a channel are added in order.
-__global__ __launch_bounds__(256) void k_rope_dw(const float* parts, int nblocks, int M, void* dwq, void* dwk, int w_dtype) {
-  __shared__ float red[16][17];
+// rows i, i + 64, ... of its channel, four at a time, then 64 sums of a channel meet in LDS.  Up to 1024 rows: 16 loads of a
+// thread, all under way together (the pass is one trip to L2 long, not its bytes).
+__global__ __launch_bounds__(1024) void k_rope_dw(const float* parts, int nblocks, int M, void* dwq, void* dwk, int w_dtype) {
+  __shared__ float red[64][17];
   void* dw = blockIdx.y ? dwk : dwq;
   if (!dw) return;                                     // (uniform over the workgroup)
   const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float s = 0.f;
-  if (c < M)
-    for (int i = sl; i < nblocks; i += 16) s += parts[((int64_t)blockIdx.y * nblocks + i) * M + c];
+  if (c < M) {
+    const float* at = parts + (int64_t)blockIdx.y * nblocks * M + c;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = sl + 64 * i;
+      v[i] = row < nblocks ? at[(int64_t)row * M] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) s += (v[i] + v[i + 1]) + (v[i + 2] + v[i + 3]);
+  }
   red[sl][cl] = s;
   __syncthreads();
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) {
+    if (sl < k) red[sl][cl] += red[sl + k][cl];
+    __syncthreads();
+  }
   if (sl == 0 && c < M) {
-    for (int i = 1; i < 16; ++i) s += red[i][cl];
+    s = red[0][cl];
     if (w_dtype == VIL_DTYPE_F32) ((float*)dw)[c] = s;
     else if (w_dtype == VIL_DTYPE_BF16) ((__bf16*)dw)[c] = (__bf16)s;
     else ((_Float16*)dw)[c] = (_Float16)s;
   }
 }
 
+constexpr int RO_BWD_BLOCKS = 1024;                    // workgroups of one side at the most: rows of partial sums (k_rope_dw reads 16 x 64)
+
 // ---- tiled kernels: heads whose halves come in chunks of CH channels that a lane loads at once (16 bytes, or 8).
 // A lane owns CH pairs of a head row: two chunks, R apart (half) or side by side (interleaved, and channels that pass
 // through), so that a rotation needs no other lane and a row's statistics meet in LPR = M / (2 CH) neighbouring lanes
-// (rounded up to a power of two).  A workgroup takes a tile of tokens with all their heads: the angles of a token are taken once,
-// into LDS, while the first loads are under way, and serve every head.
+// (rounded up to a power of two).  A workgroup takes a tile of tokens of one segment with all their heads, q's then k's; the
+// angles of a token are taken once, into LDS, and serve every head of q and k.  Segments are the images; where all share
+// their positions a workgroup walks several of them with the same angles.  Where a tensor's images follow each other
+// (stride of an image = N tokens) and positions are each image's own, all tokens are one segment, so that short images fill a tile.
+// Addresses: a scalar base per segment and 32-bit byte offsets inside the tile (products of 24-bit factors).
 template <typename T, int CH> using ro_vec = T __attribute__((ext_vector_type(CH)));
 
 __device__ __forceinline__ unsigned ro_div(unsigned x, unsigned d, unsigned magic) { return magic ? __umulhi(x, magic) : x / d; }
@@ -211,142 +234,149 @@ template <int LPR> __device__ __forceinline__ float ro_lane_sum(float v) {
   return v;
 }
 
-// where token tt of the tile that starts at token (b0, n0) lies
-__device__ __forceinline__ void ro_token(const RoParams& p, int b0, int n0, int tt, int& b, int& n) {
-  const unsigned x = (unsigned)(n0 + tt), q = ro_div(x, p.N, p.n_magic);
-  b = b0 + (int)q;
-  n = (int)(x - q * p.N);
-}
-
-// cosines and sines of a tile, trig[tt * R + j]
-__device__ __forceinline__ void ro_tile_angles(const RoParams& p, float2* trig, int b0, int n0, int ntok) {
+// cosines and sines of the tile's tokens, trig[tt * R + j]
+__device__ __forceinline__ void ro_tile_angles(const RoParams& p, float2* trig, int seg, int64_t t0, int ntok) {
+  // (a segment of its own per image: image seg, token t0 + tt; one segment of all: token t0 + tt counted through the images)
+  const int b0 = p.flat ? (int)(t0 / p.N) : seg, n0 = p.flat ? (int)(t0 - (int64_t)b0 * p.N) : (int)t0;
   for (int e = threadIdx.x; e < ntok * p.R; e += RO_THREADS) {
     const int tt = (int)ro_div(e, p.R, p.r_magic), j = e - tt * p.R;
-    int b, n;
-    ro_token(p, b0, n0, tt, b, n);
+    int b = b0, n = n0 + tt;
+    if (p.flat) {
+      const int q = (int)ro_div(n, p.N, p.n_magic);
+      b += q;
+      n -= q * p.N;
+    }
     float sn, cs;
     ro_sincos(p, b, n, j, sn, cs);
-    trig[e] = make_float2(cs, sn);
+    trig[e] = make_float2(cs, sn * p.sign);
   }
 }
 
 // a lane's pairs: chunk a at channel ca, chunk b at cb; HALF pairs a[i] with b[i], INTERLEAVED neighbours
 struct RoUnit { int ca, cb, j0; bool on, turns; };
-template <int CH> __device__ __forceinline__ RoUnit ro_unit(const RoParams& p, int sub) {
+template <int CH, bool INTER> __device__ __forceinline__ RoUnit ro_unit(const RoParams& p, int sub) {
   RoUnit u;
   u.on = sub * 2 * CH < p.M;
   u.j0 = sub * CH;
   u.turns = u.on && u.j0 < p.R;
-  const bool apart = u.turns && !p.interleaved;
+  const bool apart = u.turns && !INTER;
   u.ca = u.on ? (apart ? u.j0 : 2 * u.j0) : 0;
   u.cb = u.on ? (apart ? p.R + u.j0 : 2 * u.j0 + CH) : CH;
   return u;
 }
 
-template <int CH>
-__device__ __forceinline__ void ro_turn(float (&a)[CH], float (&b)[CH], const float2* cs, bool interleaved, float sign) {
-  if (!interleaved) {
+// cs: CH pairs (cos, sin), 32-byte aligned
+template <int CH, bool INTER>
+__device__ __forceinline__ void ro_turn(float (&a)[CH], float (&b)[CH], const float4* cs) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const float2 t = cs[i];
-      const float sn = t.y * sign, x = a[i] * t.x - b[i] * sn;
-      b[i] = b[i] * t.x + a[i] * sn;
-      a[i] = x;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; i += 2) {
-      const float2 t = cs[i / 2], v = cs[CH / 2 + i / 2];
-      const float ts = t.y * sign, vs = v.y * sign, x = a[i] * t.x - a[i + 1] * ts, y = b[i] * v.x - b[i + 1] * vs;
-      a[i + 1] = a[i + 1] * t.x + a[i] * ts;
-      a[i] = x;
-      b[i + 1] = b[i + 1] * v.x + b[i] * vs;
-      b[i] = y;
-    }
+  for (int i = 0; i < CH; i += 2) {
+    const float4 t = cs[i / 2];                  // cos, sin of pairs i, i + 1 of the lane
+    float x0, y0, x1, y1;
+    if (!INTER) { x0 = a[i]; y0 = b[i]; x1 = a[i + 1]; y1 = b[i + 1]; }
+    else if (i < CH / 2) { x0 = a[2 * i]; y0 = a[2 * i + 1]; x1 = a[2 * i + 2]; y1 = a[2 * i + 3]; }
+    else { x0 = b[2 * i - CH]; y0 = b[2 * i + 1 - CH]; x1 = b[2 * i + 2 - CH]; y1 = b[2 * i + 3 - CH]; }
+    const float u0 = x0 * t.x - y0 * t.y, v0 = y0 * t.x + x0 * t.y, u1 = x1 * t.z - y1 * t.w, v1 = y1 * t.z + x1 * t.w;
+    if (!INTER) { a[i] = u0; b[i] = v0; a[i + 1] = u1; b[i + 1] = v1; }
+    else if (i < CH / 2) { a[2 * i] = u0; a[2 * i + 1] = v0; a[2 * i + 2] = u1; a[2 * i + 3] = v1; }
+    else { b[2 * i - CH] = u0; b[2 * i + 1 - CH] = v0; b[2 * i + 2 - CH] = u1; b[2 * i + 3 - CH] = v1; }
   }
+}
+
+template <typename T, int CH> __device__ __forceinline__ ro_vec<T, CH> ro_load(const char* base, unsigned off) {
+  return *(const ro_vec<T, CH>*)(base + off);
+}
+template <typename T, int CH> __device__ __forceinline__ void ro_store(char* base, unsigned off, const float (&v)[CH]) {
+  ro_vec<T, CH> o;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) o[c] = (T)v[c];
+  *(ro_vec<T, CH>*)(base + off) = o;
 }
 
 // The forward pass; without the norm the backward pass too (sign -1).
-template <typename T, int CH, int LPR, bool NORM>
-__global__ __launch_bounds__(RO_THREADS) void k_rope_tile(RoParams p) {
-  constexpr int ROWS = RO_THREADS / LPR, IPT = 4;
-  extern __shared__ float ro_lds[];
-  float* wl = ro_lds;                                            // (2, M) weights of q, k
-  float2* trig = (float2*)(ro_lds + (NORM ? 2 * p.M : 0));
+template <typename T, int CH, int LPR, bool NORM, bool INTER>
+__global__ __launch_bounds__(RO_THREADS, NORM ? 5 : 6) void k_rope_tile(RoParams p) {
+  constexpr int ROWS = RO_THREADS / LPR, IPT = 2, SZ = sizeof(T);
+  extern __shared__ float4 ro_lds4[];
+  float* wl = (float*)ro_lds4;                                   // (2, M) weights of q, k
+  float2* trig = (float2*)(wl + (NORM ? 2 * p.M : 0));
   const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR;
   const int64_t t0 = (int64_t)blockIdx.x * p.tile;
-  const int b0 = (int)(t0 / p.N), n0 = (int)(t0 - (int64_t)b0 * p.N);
-  const int64_t left = (int64_t)p.B * p.N - t0;
-  const int ntok = left < p.tile ? (int)left : p.tile, HH = p.s[0].H + p.s[1].H, items = ntok * HH;
-  const RoUnit u = ro_unit<CH>(p, sub);
-  bool first = true;
-  for (int base = 0; base < items; base += IPT * ROWS) {
-    ro_vec<T, CH> xa[IPT], xb[IPT];
-    int tok[IPT];
-    T* y[IPT];
-    bool ok[IPT], key[IPT];
-#pragma unroll
-    for (int i = 0; i < IPT; ++i) {
-      const int idx = base + i * ROWS + slot;
-      ok[i] = idx < items && u.on;
-      const int tt = (int)ro_div(idx, HH, p.h_magic[0]), h = idx - tt * HH;
-      key[i] = h >= p.s[0].H;
-      const RoSide& S = p.s[key[i] ? 1 : 0];
-      int b, n;
-      ro_token(p, b0, n0, tt, b, n);
-      tok[i] = tt;
-      const int hs = key[i] ? h - p.s[0].H : h;
-      y[i] = (T*)S.y + b * S.y_sb + n * S.y_st + hs * S.y_sh;
-      if (ok[i]) {
-        const T* x = (const T*)S.x + b * S.x_sb + n * S.x_st + hs * S.x_sh;
-        xa[i] = *(const ro_vec<T, CH>*)(x + u.ca);
-        xb[i] = *(const ro_vec<T, CH>*)(x + u.cb);
-      }
-    }
-    if (first) {
-      first = false;
-      if (NORM)
-        for (int c = threadIdx.x; c < 2 * p.M; c += RO_THREADS) wl[c] = c < p.M ? ro_w(p.s[0].w, p.w_dtype, c) : ro_w(p.s[1].w, p.w_dtype, c - p.M);
-      ro_tile_angles(p, trig, b0, n0, ntok);
+  const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile;
+  const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
+  const RoUnit u = ro_unit<CH, INTER>(p, sub);
+  if (NORM)
+    for (int c = threadIdx.x; c < 2 * p.M; c += RO_THREADS) wl[c] = c < p.M ? ro_w(p.s[0].w, p.w_dtype, c) : ro_w(p.s[1].w, p.w_dtype, c - p.M);
+  for (int seg = seg0; seg < seg1; ++seg) {
+    if (seg == seg0 || !p.shared) {
+      if (seg != seg0) __syncthreads();                          // the last segment's angles are no longer read
+      ro_tile_angles(p, trig, seg, t0, ntok);
       __syncthreads();
     }
+    for (int side = 0; side < p.sides; ++side) {
+      const RoSide& S = p.s[side];
+      const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
+      char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
+      const unsigned xt = S.x_st * SZ, xh = S.x_sh * SZ, yt = S.y_st * SZ, yh = S.y_sh * SZ;
+      const int items = ntok * S.H;
+      float wa[CH], wb[CH];
+      if (NORM)
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) {
-      float a[CH], b[CH], r = 1.f;
+        for (int c = 0; c < CH; ++c) { wa[c] = wl[side * p.M + u.ca + c]; wb[c] = wl[side * p.M + u.cb + c]; }
+      for (int base = 0; base < items; base += IPT * ROWS) {
+        ro_vec<T, CH> xa[IPT], xb[IPT];
+        unsigned yo[IPT];
+        int tok[IPT];
+        bool ok[IPT];
 #pragma unroll
-      for (int c = 0; c < CH; ++c) { a[c] = ok[i] ? (float)xa[i][c] : 0.f; b[c] = ok[i] ? (float)xb[i][c] : 0.f; }
-      if (NORM) {
-        float s = 0.f;
+        for (int i = 0; i < IPT; ++i) {
+          const int idx = base + i * ROWS + slot;
+          ok[i] = idx < items && u.on;
+          const int tt = (int)ro_div(idx, S.H, p.h_magic[side]), h = idx - tt * S.H;
+          tok[i] = tt;
+          yo[i] = __umul24(tt, yt) + __umul24(h, yh);
+          if (ok[i]) {
+            const unsigned xo = __umul24(tt, xt) + __umul24(h, xh);
+            xa[i] = ro_load<T, CH>(x, xo + u.ca * SZ);
+            xb[i] = ro_load<T, CH>(x, xo + u.cb * SZ);
+          }
+        }
 #pragma unroll
-        for (int c = 0; c < CH; ++c) { s = fmaf(a[c], a[c], s); s = fmaf(b[c], b[c], s); }
-        r = 1.0f / sqrtf(ro_lane_sum<LPR>(s) / p.M + p.eps);
+        for (int i = 0; i < IPT; ++i) {
+          float a[CH], b[CH], r = 1.f;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) { a[c] = (float)xa[i][c]; b[c] = (float)xb[i][c]; }
+          if (NORM) {
+            float s = 0.f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) { s = fmaf(a[c], a[c], s); s = fmaf(b[c], b[c], s); }
+            if (LPR > 2 && !u.on) s = 0.f;                       // (lanes past a head that is no power of two)
+            r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s), p.inv_m, p.eps));
+#pragma unroll
+            for (int c = 0; c < CH; ++c) { a[c] = a[c] * r * wa[c]; b[c] = b[c] * r * wb[c]; }
+          }
+          if (!ok[i]) continue;
+          if (u.turns) ro_turn<CH, INTER>(a, b, (const float4*)(trig + tok[i] * p.R + u.j0));
+          ro_store<T, CH>(y, yo[i] + u.ca * SZ, a);
+          ro_store<T, CH>(y, yo[i] + u.cb * SZ, b);
+        }
       }
-      if (!ok[i]) continue;
-      if (NORM) {
-        const float* w = wl + (key[i] ? p.M : 0);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) { a[c] = a[c] * r * w[u.ca + c]; b[c] = b[c] * r * w[u.cb + c]; }
-      }
-      if (u.turns) ro_turn<CH>(a, b, trig + tok[i] * p.R + u.j0, p.interleaved, p.sign);
-      ro_vec<T, CH> oa, ob;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) { oa[c] = (T)a[c]; ob[c] = (T)b[c]; }
-      *(ro_vec<T, CH>*)(y[i] + u.ca) = oa;
-      *(ro_vec<T, CH>*)(y[i] + u.cb) = ob;
     }
   }
 }
 
-// The norm's backward pass.  blockIdx.y: q or k; a workgroup walks tiles and keeps its share of dw in registers.
-template <typename T, int CH, int LPR>
-__global__ __launch_bounds__(RO_THREADS) void k_rope_norm_bwd(RoParams p) {
-  constexpr int ROWS = RO_THREADS / LPR, IPT = 2;
-  extern __shared__ float ro_lds[];
-  float2* trig = (float2*)ro_lds;
+// The norm's backward pass.  blockIdx.z: q or k; a workgroup walks tiles and segments and keeps its share of dw in registers.
+template <typename T, int CH, int LPR, bool INTER>
+__global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
+  constexpr int ROWS = RO_THREADS / LPR, IPT = 2, SZ = sizeof(T);
+  extern __shared__ float4 ro_lds4[];
+  float2* trig = (float2*)ro_lds4;
   __shared__ float red[4][RO_M_MAX];
-  const RoSide& S = p.s[blockIdx.y];
+  const int side = blockIdx.z;
+  const RoSide& S = p.s[side];
   const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR, wave = threadIdx.x >> 6;
-  const RoUnit u = ro_unit<CH>(p, sub);
+  const RoUnit u = ro_unit<CH, INTER>(p, sub);
+  const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
+  const unsigned xt = S.x_st * SZ, xh = S.x_sh * SZ, yt = S.y_st * SZ, yh = S.y_sh * SZ, gt = S.g_st * SZ, gh = S.g_sh * SZ;
   float wa[CH], wb[CH], da[CH], db[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -356,67 +386,67 @@ __global__ __launch_bounds__(RO_THREADS) void k_rope_norm_bwd(RoParams p) {
   }
   for (int tile = blockIdx.x; tile < p.ntiles; tile += gridDim.x) {
     const int64_t t0 = (int64_t)tile * p.tile;
-    const int b0 = (int)(t0 / p.N), n0 = (int)(t0 - (int64_t)b0 * p.N);
-    const int64_t left = (int64_t)p.B * p.N - t0;
-    const int ntok = left < p.tile ? (int)left : p.tile, items = ntok * S.H;
-    bool first = true;
-    for (int base = 0; base < items; base += IPT * ROWS) {
-      ro_vec<T, CH> xa[IPT], xb[IPT], ya[IPT], yb[IPT];
-      T* o[IPT];
-      int tok[IPT];
-      bool ok[IPT];
-#pragma unroll
-      for (int i = 0; i < IPT; ++i) {
-        const int idx = base + i * ROWS + slot;
-        ok[i] = idx < items && u.on;
-        const int tt = (int)ro_div(idx, S.H, p.h_magic[blockIdx.y]), h = idx - tt * S.H;
-        int b, n;
-        ro_token(p, b0, n0, tt, b, n);
-        tok[i] = tt;
-        o[i] = (T*)S.y + b * S.y_sb + n * S.y_st + h * S.y_sh;
-        if (ok[i]) {
-          const T* x = (const T*)S.x + b * S.x_sb + n * S.x_st + h * S.x_sh;
-          const T* g = (const T*)S.g + b * S.g_sb + n * S.g_st + h * S.g_sh;
-          xa[i] = *(const ro_vec<T, CH>*)(x + u.ca);
-          xb[i] = *(const ro_vec<T, CH>*)(x + u.cb);
-          ya[i] = *(const ro_vec<T, CH>*)(g + u.ca);
-          yb[i] = *(const ro_vec<T, CH>*)(g + u.cb);
-        }
-      }
-      if (first) {
-        first = false;
-        ro_tile_angles(p, trig, b0, n0, ntok);
+    const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile, items = ntok * S.H;
+    for (int seg = seg0; seg < seg1; ++seg) {
+      if (seg == seg0 || !p.shared) {
+        __syncthreads();                                 // the angles before are no longer read
+        ro_tile_angles(p, trig, seg, t0, ntok);
         __syncthreads();
       }
+      const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
+      const char* g = (const char*)S.g + (seg * S.g_sb + t0 * S.g_st) * SZ;
+      char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
+      for (int base = 0; base < items; base += IPT * ROWS) {
+        ro_vec<T, CH> xa[IPT], xb[IPT], ya[IPT], yb[IPT];
+        unsigned yo[IPT];
+        int tok[IPT];
+        bool ok[IPT];
 #pragma unroll
-      for (int i = 0; i < IPT; ++i) {
-        float a[CH], b[CH], ga[CH], gb[CH], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          a[c] = ok[i] ? (float)xa[i][c] : 0.f; b[c] = ok[i] ? (float)xb[i][c] : 0.f;
-          ga[c] = ok[i] ? (float)ya[i][c] : 0.f; gb[c] = ok[i] ? (float)yb[i][c] : 0.f;
+        for (int i = 0; i < IPT; ++i) {
+          const int idx = base + i * ROWS + slot;
+          ok[i] = idx < items && u.on;
+          const int tt = (int)ro_div(idx, S.H, p.h_magic[side]), h = idx - tt * S.H;
+          tok[i] = tt;
+          yo[i] = __umul24(tt, yt) + __umul24(h, yh);
+          if (ok[i]) {
+            const unsigned xo = __umul24(tt, xt) + __umul24(h, xh), go = __umul24(tt, gt) + __umul24(h, gh);
+            xa[i] = ro_load<T, CH>(x, xo + u.ca * SZ);
+            xb[i] = ro_load<T, CH>(x, xo + u.cb * SZ);
+            ya[i] = ro_load<T, CH>(g, go + u.ca * SZ);
+            yb[i] = ro_load<T, CH>(g, go + u.cb * SZ);
+          }
         }
-        if (u.turns && ok[i]) ro_turn<CH>(ga, gb, trig + tok[i] * p.R + u.j0, p.interleaved, -1.0f);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          s1 = fmaf(a[c], a[c], s1); s1 = fmaf(b[c], b[c], s1);
-          s2 = fmaf(ga[c] * wa[c], a[c], s2); s2 = fmaf(gb[c] * wb[c], b[c], s2);
-        }
-        const float r = 1.0f / sqrtf(ro_lane_sum<LPR>(s1) / p.M + p.eps), m = r * r * (ro_lane_sum<LPR>(s2) / p.M);
-        if (!ok[i]) continue;
-        ro_vec<T, CH> oa, ob;
+        for (int i = 0; i < IPT; ++i) {
+          float a[CH], b[CH], ga[CH], gb[CH], s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          da[c] = fmaf(ga[c], a[c] * r, da[c]);
-          db[c] = fmaf(gb[c], b[c] * r, db[c]);
-          oa[c] = (T)(r * (ga[c] * wa[c] - a[c] * m));
-          ob[c] = (T)(r * (gb[c] * wb[c] - b[c] * m));
+          for (int c = 0; c < CH; ++c) {
+            a[c] = (float)xa[i][c]; b[c] = (float)xb[i][c];
+            ga[c] = (float)ya[i][c]; gb[c] = (float)yb[i][c];
+          }
+          if (u.turns && ok[i]) ro_turn<CH, INTER>(ga, gb, (const float4*)(trig + tok[i] * p.R + u.j0));
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            s1 = fmaf(a[c], a[c], s1); s1 = fmaf(b[c], b[c], s1);
+            s2 = fmaf(ga[c] * wa[c], a[c], s2); s2 = fmaf(gb[c] * wb[c], b[c], s2);
+          }
+          if (LPR > 2 && !u.on) s1 = s2 = 0.f;
+          const float r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s1), p.inv_m, p.eps));
+          const float m = r * r * r * (ro_lane_sum<LPR>(s2) * p.inv_m);
+          if (!ok[i]) continue;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            ga[c] *= r; gb[c] *= r;
+            da[c] = fmaf(ga[c], a[c], da[c]);
+            db[c] = fmaf(gb[c], b[c], db[c]);
+            a[c] = ga[c] * wa[c] - a[c] * m;
+            b[c] = gb[c] * wb[c] - b[c] * m;
+          }
+          ro_store<T, CH>(y, yo[i] + u.ca * SZ, a);
+          ro_store<T, CH>(y, yo[i] + u.cb * SZ, b);
         }
-        *(ro_vec<T, CH>*)(o[i] + u.ca) = oa;
-        *(ro_vec<T, CH>*)(o[i] + u.cb) = ob;
       }
     }
-    __syncthreads();                                   // the next tile's angles overwrite this one's
   }
   if (!p.parts) return;
 #pragma unroll
@@ -426,8 +456,9 @@ __global__ __launch_bounds__(RO_THREADS) void k_rope_norm_bwd(RoParams p) {
     if ((threadIdx.x & 63) < LPR && u.on) { red[wave][u.ca + c] = da[c]; red[wave][u.cb + c] = db[c]; }
   }
   __syncthreads();
+  const int64_t row = (int64_t)side * p.nblocks + blockIdx.y * gridDim.x + blockIdx.x;
   for (int c = threadIdx.x; c < p.M; c += RO_THREADS)
-    p.parts[((int64_t)blockIdx.y * p.nblocks + blockIdx.x) * p.M + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+    p.parts[row * p.M + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
 }
 
 unsigned ro_magic(int64_t most, int64_t d) {           // x / d == umulhi(x, magic) for every x <= most, else 0
@@ -437,108 +468,128 @@ unsigned ro_magic(int64_t most, int64_t d) {           // x / d == umulhi(x, mag
 }
 
 // Channels of a chunk: 16 bytes where the head, the rotated part and every stride and address allow it, else 8 bytes of a 16-bit
-// type, else 0: one element at a time.
+// type, else 0: one element at a time (as where a token or head stride passes the 24 bits of a factor).
 int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
   const int size = dtype == VIL_DTYPE_F32 ? 4 : 2;
   for (int ch = 16 / size; ch >= 4; ch /= 2) {
     if (p.M % (2 * ch) || p.R % ch) continue;
     uintptr_t bits = 0;
+    bool small = true;
     for (int i = 0; i < 2; ++i) {
       const RoSide& S = p.s[i];
       if (!S.H) continue;
-      bits |= (uintptr_t)S.x | (uintptr_t)S.y | (uintptr_t)(S.x_sb | S.x_st | S.x_sh | S.y_sb | S.y_st | S.y_sh) * size;
-      if (bwd_norm) bits |= (uintptr_t)S.g | (uintptr_t)(S.g_sb | S.g_st | S.g_sh) * size;
+      const int64_t strides[6] = {S.x_st, S.x_sh, S.y_st, S.y_sh, bwd_norm ? S.g_st : 0, bwd_norm ? S.g_sh : 0};
+      for (int64_t st : strides) {
+        bits |= (uintptr_t)(st * size);
+        small = small && st >= 0 && st * size < (1 << 24);
+      }
+      // (offsets in a tile stay under 2^32: the heads under 2^30 here, the tokens in ro_plan)
+      small = small && S.H * S.x_sh * size < (1 << 30) && S.H * S.y_sh * size < (1 << 30) && (!bwd_norm || S.H * S.g_sh * size < (1 << 30));
+      bits |= (uintptr_t)S.x | (uintptr_t)S.y | (uintptr_t)((S.x_sb | S.y_sb) * size);
+      if (bwd_norm) bits |= (uintptr_t)S.g | (uintptr_t)(S.g_sb * size);
     }
-    if (bits % (ch * size) == 0) return ch;
+    if (small && bits % (ch * size) == 0) return ch;
   }
   return 0;
 }
 
-// tokens of a tile: `ipt` head rows to a thread, angles in 16 KB, and no larger than leaves `want` tiles
-int ro_tile(const RoParams& p, int lpr, int heads, int ipt, int64_t want) {
+// Tiles and segments of a launch: `rows` head rows of one side to a workgroup at the most, angles in 16 KB, and at least `want`
+// workgroups where there is work for them.
+void ro_plan(RoParams& p, int size, int rows, int64_t want) {
+  bool flat = true;                                    // images follow each other in every tensor
+  int64_t st = 1;
+  for (int i = 0; i < p.sides; ++i) {
+    const RoSide& S = p.s[i];
+    flat = flat && S.x_sb == p.N * S.x_st && S.y_sb == p.N * S.y_st && (!S.g || S.g_sb == p.N * S.g_st);
+    for (int64_t v : {S.x_st, S.y_st, S.g ? S.g_st : 0}) st = v > st ? v : st;
+  }
+  const bool shared = p.R == 0 || p.pos_sb == 0 || p.B == 1;
+  const int H = p.s[0].H > p.s[1].H ? p.s[0].H : p.s[1].H;
+  int64_t tile = rows / H;
+  if (tile > 512) tile = 512;
+  if (p.R > 0 && tile > 2048 / p.R) tile = 2048 / p.R;
+  if (tile > (1 << 30) / (st * size)) tile = (1 << 30) / (st * size);
   const int64_t tokens = (int64_t)p.B * p.N;
-  int64_t t = (int64_t)ipt * (RO_THREADS / lpr) / heads;
-  if (p.R > 0 && t > 2048 / p.R) t = 2048 / p.R;
-  if (t > (tokens + want - 1) / want) t = (tokens + want - 1) / want;
-  return t < 1 ? 1 : (int)t;
+  if (tile > (tokens + want - 1) / want) tile = (tokens + want - 1) / want;
+  if (tile < 1) tile = 1;
+  // one segment of all tokens for positions of each image's own, and for images shorter than a tile
+  p.flat = flat && p.B > 1 && (!shared || p.N < tile);
+  p.nseg = p.flat ? 1 : p.B;
+  p.T = p.flat ? tokens : p.N;
+  if (tile > p.T) tile = p.T;
+  p.tile = (int)tile;
+  p.ntiles = (int)((p.T + tile - 1) / tile);
+  p.spg = 1;
+  p.shared = shared;
+  if (shared && p.nseg > 1) {
+    const int64_t units = (int64_t)p.ntiles * p.nseg, spg = units / want;
+    p.spg = spg < 1 ? 1 : spg > p.nseg ? p.nseg : (int)spg;
+  }
+  for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic((int64_t)p.tile * p.s[i].H + 2 * RO_THREADS, p.s[i].H);
+  p.n_magic = ro_magic((int64_t)p.N + p.tile, p.N);
+  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
 }
 
 template <typename T, int CH, int LPR, bool NORM>
 int ro_tile_launch(RoParams& p, hipStream_t s) {
-  const int HH = p.s[0].H + p.s[1].H;
-  p.tile = ro_tile(p, LPR, HH, 4, 1024);
-  p.h_magic[0] = ro_magic((int64_t)p.tile * HH + 4 * RO_THREADS, HH);
-  p.n_magic = ro_magic((int64_t)p.N + p.tile + 4 * RO_THREADS, p.N);
-  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
-  const int64_t tiles = ((int64_t)p.B * p.N + p.tile - 1) / p.tile;
-  const size_t lds = (NORM ? 2 * p.M * sizeof(float) : 0) + (size_t)p.tile * p.R * sizeof(float2);
-  k_rope_tile<T, CH, LPR, NORM><<<dim3((unsigned)tiles), dim3(RO_THREADS), lds, s>>>(p);
+  ro_plan(p, sizeof(T), 4 * RO_THREADS / LPR, 1536);
+  if (p.nseg > 65535 * (int64_t)p.spg) p.spg = (p.nseg + 65534) / 65535;         // (the grid's second axis)
+  const dim3 grid(p.ntiles, (p.nseg + p.spg - 1) / p.spg), block(RO_THREADS);
+  const size_t lds = (size_t)p.tile * p.R * sizeof(float2) + (NORM ? 2 * p.M * sizeof(float) : 0);
+  if (p.interleaved) k_rope_tile<T, CH, LPR, NORM, true><<<grid, block, lds, s>>>(p);
+  else k_rope_tile<T, CH, LPR, NORM, false><<<grid, block, lds, s>>>(p);
   return (int)hipGetLastError();
 }
-
-constexpr int RO_BWD_BLOCKS = 1024;                    // workgroups of one side at the most: rows of partial sums
 
 template <typename T, int CH, int LPR>
-int ro_bwd_launch(RoParams& p, int sides, hipStream_t s) {
-  const int H = p.s[0].H > p.s[1].H ? p.s[0].H : p.s[1].H;
-  p.tile = ro_tile(p, LPR, H, 2, 1024);
-  for (int i = 0; i < sides; ++i) p.h_magic[i] = ro_magic((int64_t)p.tile * p.s[i].H + 2 * RO_THREADS, p.s[i].H);
-  p.n_magic = ro_magic((int64_t)p.N + p.tile + 2 * RO_THREADS, p.N);
-  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
-  p.ntiles = (int)(((int64_t)p.B * p.N + p.tile - 1) / p.tile);
-  p.nblocks = p.ntiles < RO_BWD_BLOCKS ? p.ntiles : RO_BWD_BLOCKS;
-  k_rope_norm_bwd<T, CH, LPR><<<dim3(p.nblocks, sides), dim3(RO_THREADS), (size_t)p.tile * p.R * sizeof(float2), s>>>(p);
+int ro_bwd_launch(RoParams& p, hipStream_t s) {
+  ro_plan(p, sizeof(T), 4 * RO_THREADS / LPR, RO_BWD_BLOCKS);
+  if (p.nseg > RO_BWD_BLOCKS * (int64_t)p.spg) p.spg = (p.nseg + RO_BWD_BLOCKS - 1) / RO_BWD_BLOCKS;   // (short images)
+  const int groups = (p.nseg + p.spg - 1) / p.spg, x = RO_BWD_BLOCKS / groups;
+  const dim3 grid(x < p.ntiles ? x : p.ntiles, groups, p.sides), block(RO_THREADS);
+  p.nblocks = grid.x * grid.y;
+  const size_t lds = (size_t)p.tile * p.R * sizeof(float2);
+  if (p.interleaved) k_rope_norm_bwd<T, CH, LPR, true><<<grid, block, lds, s>>>(p);
+  else k_rope_norm_bwd<T, CH, LPR, false><<<grid, block, lds, s>>>(p);
   return (int)hipGetLastError();
 }
 
-template <typename T, int CH, bool NORM>
-int ro_tile_lanes(RoParams& p, hipStream_t s) {
+template <typename T, int CH, bool NORM, bool BWD>
+int ro_lanes(RoParams& p, hipStream_t s) {
   const int lanes = p.M / (2 * CH);
-  if (lanes <= 1) return ro_tile_launch<T, CH, 1, NORM>(p, s);
-  if (lanes <= 2) return ro_tile_launch<T, CH, 2, NORM>(p, s);
-  if (lanes <= 4) return ro_tile_launch<T, CH, 4, NORM>(p, s);
-  if (lanes <= 8) return ro_tile_launch<T, CH, 8, NORM>(p, s);
-  if (lanes <= 16) return ro_tile_launch<T, CH, 16, NORM>(p, s);
-  return ro_tile_launch<T, CH, 32, NORM>(p, s);
-}
-template <typename T, int CH>
-int ro_bwd_lanes(RoParams& p, int sides, hipStream_t s) {
-  const int lanes = p.M / (2 * CH);
-  if (lanes <= 1) return ro_bwd_launch<T, CH, 1>(p, sides, s);
-  if (lanes <= 2) return ro_bwd_launch<T, CH, 2>(p, sides, s);
-  if (lanes <= 4) return ro_bwd_launch<T, CH, 4>(p, sides, s);
-  if (lanes <= 8) return ro_bwd_launch<T, CH, 8>(p, sides, s);
-  if (lanes <= 16) return ro_bwd_launch<T, CH, 16>(p, sides, s);
-  return ro_bwd_launch<T, CH, 32>(p, sides, s);
+#define RO_LANES(L)                                                   \
+  if (lanes <= L) {                                                   \
+    if constexpr (NORM && BWD) return ro_bwd_launch<T, CH, L>(p, s);  \
+    else return ro_tile_launch<T, CH, L, NORM>(p, s);                 \
+  }
+  RO_LANES(1) RO_LANES(2) RO_LANES(4) RO_LANES(8) RO_LANES(16)
+  if constexpr (CH == 4) { RO_LANES(32) }
+#undef RO_LANES
+  return VIL_E_HEAD_DIM;                                               // (not reached: M <= 256)
 }
 template <typename T, bool NORM, bool BWD>
-int ro_tiled(RoParams& p, int ch, int sides, hipStream_t s) {
-  if constexpr (NORM && BWD) {
-    if constexpr (sizeof(T) == 2)
-      if (ch == 8) return ro_bwd_lanes<T, 8>(p, sides, s);
-    return ro_bwd_lanes<T, 4>(p, sides, s);
-  } else {
-    p.sign = BWD ? -1.0f : 1.0f;
-    if constexpr (sizeof(T) == 2)
-      if (ch == 8) return ro_tile_lanes<T, 8, NORM>(p, s);
-    return ro_tile_lanes<T, 4, NORM>(p, s);
-  }
+int ro_tiled(RoParams& p, int ch, hipStream_t s) {
+  p.sign = BWD ? -1.0f : 1.0f;
+  if constexpr (sizeof(T) == 2)
+    if (ch == 8) return ro_lanes<T, 8, NORM, BWD>(p, s);
+  return ro_lanes<T, 4, NORM, BWD>(p, s);
 }
 
+// k_rope_any: lanes of a head row, workgroups of a side
+int ro_lpr(int M) { return M <= 16 ? 8 : M <= 32 ? 16 : M <= 64 ? 32 : 64; }
 int ro_nblocks(const VilRopeDesc* d, int lpr) {
   const int64_t rows = (int64_t)d->B * d->N * (d->Hq > d->Hk ? d->Hq : d->Hk);
   const int64_t need = (rows + 4 * (64 / lpr) - 1) / (4 * (64 / lpr));
-  return (int)(need < 1024 ? (need < 1 ? 1 : need) : 1024);
+  return (int)(need < RO_BWD_BLOCKS ? (need < 1 ? 1 : need) : RO_BWD_BLOCKS);
 }
-
-int ro_lpr(int M) { return M <= 16 ? 8 : M <= 32 ? 16 : M <= 64 ? 32 : 64; }
 
 template <typename T, bool NORM, bool BWD>
 int ro_launch(RoParams& p, int dtype, int sides, hipStream_t s) {
   // (without the norm the backward pass reads g alone)
   if (BWD && !NORM)
     for (int i = 0; i < 2; ++i) { p.s[i].x = p.s[i].g; p.s[i].x_sb = p.s[i].g_sb; p.s[i].x_st = p.s[i].g_st; p.s[i].x_sh = p.s[i].g_sh; }
-  if (const int ch = ro_chunk(p, dtype, NORM && BWD)) return ro_tiled<T, NORM, BWD>(p, ch, sides, s);
+  p.sides = sides;
+  if (const int ch = ro_chunk(p, dtype, NORM && BWD)) return ro_tiled<T, NORM, BWD>(p, ch, s);
   const dim3 grid(p.nblocks, sides), block(RO_THREADS);
   const int pairs = p.M / 2;
   if (pairs <= 8) k_rope_any<T, 8, 1, NORM, BWD><<<grid, block, 0, s>>>(p);
@@ -592,6 +643,7 @@ void ro_fill(RoParams& p, const VilRopeDesc* d, const void* pos, const void* fre
   p.axes = d->axes;
   for (int a = 0, e = 0; a < RO_AXES; ++a) p.sec_end[a] = e += a < d->axes ? d->sections[a] : 0;
   p.eps = d->eps;
+  p.inv_m = 1.0f / d->M;
   p.s[0].H = d->Hq; p.s[1].H = d->Hk;
 }
 #define RO_STRIDES(SIDE, F, NAME) SIDE.F##_sb = d->NAME##_sb, SIDE.F##_st = d->NAME##_st, SIDE.F##_sh = d->NAME##_sh
@@ -642,7 +694,7 @@ extern "C" int vil_qk_rope_bwd(const VilRopeDesc* d, const void* gq, const void*
   if (!empty)
     if (int e = ro_dispatch<true>(d, p, (hipStream_t)stream)) return e;
   if (dw) {                                   // (an empty batch: zeros)
-    k_rope_dw<<<dim3((d->M + 15) / 16, 2), dim3(256), 0, (hipStream_t)stream>>>((const float*)workspace, p.nblocks, d->M, dwq, dwk, d->w_dtype);
+    k_rope_dw<<<dim3((d->M + 15) / 16, 2), dim3(1024), 0, (hipStream_t)stream>>>((const float*)workspace, p.nblocks, d->M, dwq, dwk, d->w_dtype);
     return (int)hipGetLastError();
   }
   return VIL_OK;
