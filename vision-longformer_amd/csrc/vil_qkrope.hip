@@ -34,7 +34,7 @@ struct RoParams {
   int axes, sec_end[RO_AXES];
   float eps, sign;            // sign: +1 rotates by theta, -1 back
   // tiled kernels: tokens of a tile, tiles of a segment, segments, segments of a workgroup, tokens of a segment; magic numbers of
-  // x / H, x / N, x / R (0: divide)
+  // x / H, x / N, x / R
   int sides, tile, ntiles, nseg, spg, flat, shared;
   int64_t T;
   unsigned h_magic[2], n_magic, r_magic;
@@ -219,7 +219,8 @@ constexpr int RO_BWD_BLOCKS = 1024;                    // workgroups of one side
 // Addresses: a scalar base per segment and 32-bit byte offsets inside the tile (products of 24-bit factors).
 template <typename T, int CH> using ro_vec = T __attribute__((ext_vector_type(CH)));
 
-__device__ __forceinline__ unsigned ro_div(unsigned x, unsigned d, unsigned magic) { return magic ? __umulhi(x, magic) : x / d; }
+// x / d for x d < 2^31, magic = ceil(2^31 / d): the excess x (magic d - 2^31) < x d stays under 2^31
+__device__ __forceinline__ unsigned ro_div(unsigned x, unsigned magic) { return __umulhi(2 * x, magic); }
 
 template <int CTRL> __device__ __forceinline__ float ro_dpp(float v) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
@@ -239,10 +240,10 @@ __device__ __forceinline__ void ro_tile_angles(const RoParams& p, float2* trig, 
   // (a segment of its own per image: image seg, token t0 + tt; one segment of all: token t0 + tt counted through the images)
   const int b0 = p.flat ? (int)(t0 / p.N) : seg, n0 = p.flat ? (int)(t0 - (int64_t)b0 * p.N) : (int)t0;
   for (int e = threadIdx.x; e < ntok * p.R; e += RO_THREADS) {
-    const int tt = (int)ro_div(e, p.R, p.r_magic), j = e - tt * p.R;
+    const int tt = (int)ro_div(e, p.r_magic), j = e - tt * p.R;
     int b = b0, n = n0 + tt;
     if (p.flat) {
-      const int q = (int)ro_div(n, p.N, p.n_magic);
+      const int q = p.n_magic ? (int)ro_div(n, p.n_magic) : n >= p.N;   // (0: an image is no shorter than a tile)
       b += q;
       n -= q * p.N;
     }
@@ -292,57 +293,75 @@ template <typename T, int CH> __device__ __forceinline__ void ro_store(char* bas
   *(ro_vec<T, CH>*)(base + off) = o;
 }
 
+// Head rows of a tile, one side: IPT rows to a thread and step, the next step's loads issued before this one's arithmetic, so that
+// loads stay under way while a wave computes (without it the forward pass took 82 us where a copy of the same slices takes 61).
+// Rows past the end load the last row again and store nothing.
+template <typename T, int CH, int LPR, int IPT> struct RoRows {
+  static constexpr int ROWS = RO_THREADS / LPR;
+  int items, H;
+  unsigned magic;
+  __device__ __forceinline__ void at(int base, int i, int& tt, int& h, bool& ok) const {
+    int idx = base + i * ROWS + (int)threadIdx.x / LPR;
+    ok = idx < items;
+    idx = ok ? idx : items - 1;
+    tt = (int)ro_div(idx, magic);
+    h = idx - tt * H;
+  }
+};
+
 // The forward pass; without the norm the backward pass too (sign -1).
 template <typename T, int CH, int LPR, bool NORM, bool INTER>
-__global__ __launch_bounds__(RO_THREADS, NORM ? 5 : 6) void k_rope_tile(RoParams p) {
-  constexpr int ROWS = RO_THREADS / LPR, IPT = 2, SZ = sizeof(T);
+__global__ __launch_bounds__(RO_THREADS, NORM ? 4 : 5) void k_rope_tile(RoParams p) {
+  constexpr int IPT = 2, STEP = IPT * RO_THREADS / LPR, SZ = sizeof(T);
   extern __shared__ float4 ro_lds4[];
   float* wl = (float*)ro_lds4;                                   // (2, M) weights of q, k
   float2* trig = (float2*)(wl + (NORM ? 2 * p.M : 0));
-  const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR;
   const int64_t t0 = (int64_t)blockIdx.x * p.tile;
   const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile;
   const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
-  const RoUnit u = ro_unit<CH, INTER>(p, sub);
+  const RoUnit u = ro_unit<CH, INTER>(p, threadIdx.x % LPR);
   if (NORM)
     for (int c = threadIdx.x; c < 2 * p.M; c += RO_THREADS) wl[c] = c < p.M ? ro_w(p.s[0].w, p.w_dtype, c) : ro_w(p.s[1].w, p.w_dtype, c - p.M);
-  for (int seg = seg0; seg < seg1; ++seg) {
-    if (seg == seg0 || !p.shared) {
-      if (seg != seg0) __syncthreads();                          // the last segment's angles are no longer read
-      ro_tile_angles(p, trig, seg, t0, ntok);
-      __syncthreads();
-    }
+  const int run = p.shared ? seg1 - seg0 : 1;                    // segments that the same angles serve
+  for (int first = seg0; first < seg1; first += run) {
+    if (first != seg0) __syncthreads();                          // the angles before are no longer read
+    ro_tile_angles(p, trig, first, t0, ntok);
+    __syncthreads();
     for (int side = 0; side < p.sides; ++side) {
       const RoSide& S = p.s[side];
-      const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
-      char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
       const unsigned xt = S.x_st * SZ, xh = S.x_sh * SZ, yt = S.y_st * SZ, yh = S.y_sh * SZ;
-      const int items = ntok * S.H;
+      const RoRows<T, CH, LPR, IPT> rows = {ntok * S.H, S.H, p.h_magic[side]};
       float wa[CH], wb[CH];
       if (NORM)
 #pragma unroll
         for (int c = 0; c < CH; ++c) { wa[c] = wl[side * p.M + u.ca + c]; wb[c] = wl[side * p.M + u.cb + c]; }
-      for (int base = 0; base < items; base += IPT * ROWS) {
-        ro_vec<T, CH> xa[IPT], xb[IPT];
-        unsigned yo[IPT];
-        int tok[IPT];
-        bool ok[IPT];
+      ro_vec<T, CH> xa[IPT], xb[IPT], na[IPT], nb[IPT];
+      const auto load = [&](int seg, int base, ro_vec<T, CH>(&va)[IPT], ro_vec<T, CH>(&vb)[IPT]) {
+        const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
 #pragma unroll
         for (int i = 0; i < IPT; ++i) {
-          const int idx = base + i * ROWS + slot;
-          ok[i] = idx < items && u.on;
-          const int tt = (int)ro_div(idx, S.H, p.h_magic[side]), h = idx - tt * S.H;
-          tok[i] = tt;
-          yo[i] = __umul24(tt, yt) + __umul24(h, yh);
-          if (ok[i]) {
-            const unsigned xo = __umul24(tt, xt) + __umul24(h, xh);
-            xa[i] = ro_load<T, CH>(x, xo + u.ca * SZ);
-            xb[i] = ro_load<T, CH>(x, xo + u.cb * SZ);
-          }
+          int tt, h;
+          bool ok;
+          rows.at(base, i, tt, h, ok);
+          const unsigned xo = __umul24(tt, xt) + __umul24(h, xh);
+          va[i] = ro_load<T, CH>(x, xo + u.ca * SZ);
+          vb[i] = ro_load<T, CH>(x, xo + u.cb * SZ);
         }
+      };
+      int seg = first, base = 0;
+      load(seg, 0, xa, xb);
+      for (;;) {
+        int nseg = seg, nbase = base + STEP;
+        if (nbase >= rows.items) { nbase = 0; ++nseg; }
+        const bool more = nseg < first + run;
+        if (more) load(nseg, nbase, na, nb);
+        char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
 #pragma unroll
         for (int i = 0; i < IPT; ++i) {
-          float a[CH], b[CH], r = 1.f;
+          int tt, h;
+          bool ok;
+          rows.at(base, i, tt, h, ok);
+          float a[CH], b[CH];
 #pragma unroll
           for (int c = 0; c < CH; ++c) { a[c] = (float)xa[i][c]; b[c] = (float)xb[i][c]; }
           if (NORM) {
@@ -350,90 +369,107 @@ __global__ __launch_bounds__(RO_THREADS, NORM ? 5 : 6) void k_rope_tile(RoParams
 #pragma unroll
             for (int c = 0; c < CH; ++c) { s = fmaf(a[c], a[c], s); s = fmaf(b[c], b[c], s); }
             if (LPR > 2 && !u.on) s = 0.f;                       // (lanes past a head that is no power of two)
-            r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s), p.inv_m, p.eps));
+            const float r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s), p.inv_m, p.eps));
 #pragma unroll
             for (int c = 0; c < CH; ++c) { a[c] = a[c] * r * wa[c]; b[c] = b[c] * r * wb[c]; }
           }
-          if (!ok[i]) continue;
-          if (u.turns) ro_turn<CH, INTER>(a, b, (const float4*)(trig + tok[i] * p.R + u.j0));
-          ro_store<T, CH>(y, yo[i] + u.ca * SZ, a);
-          ro_store<T, CH>(y, yo[i] + u.cb * SZ, b);
+          if (u.turns) ro_turn<CH, INTER>(a, b, (const float4*)(trig + tt * p.R + u.j0));
+          if (ok && u.on) {
+            const unsigned yo = __umul24(tt, yt) + __umul24(h, yh);
+            ro_store<T, CH>(y, yo + u.ca * SZ, a);
+            ro_store<T, CH>(y, yo + u.cb * SZ, b);
+          }
         }
+        if (!more) break;
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) { xa[i] = na[i]; xb[i] = nb[i]; }
+        seg = nseg;
+        base = nbase;
       }
     }
   }
 }
 
+// sum over the lanes of 16 that share lane % LPR, in all of them
+template <int LPR> __device__ __forceinline__ float ro_row_of_16(float v) {
+  if (LPR <= 8) v += ro_dpp<0x128>(v);          // row_ror 8
+  if (LPR <= 4) v += ro_dpp<0x124>(v);
+  if (LPR <= 2) v += ro_dpp<0x122>(v);
+  if (LPR <= 1) v += ro_dpp<0x121>(v);
+  return v;
+}
+
 // The norm's backward pass.  blockIdx.z: q or k; a workgroup walks tiles and segments and keeps its share of dw in registers.
 template <typename T, int CH, int LPR, bool INTER>
 __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
-  constexpr int ROWS = RO_THREADS / LPR, IPT = 2, SZ = sizeof(T);
-  extern __shared__ float4 ro_lds4[];
+  constexpr int STEP = RO_THREADS / LPR, SZ = sizeof(T);
+  extern __shared__ float4 ro_lds4[];                  // the weights; a tile's angles; at the end 16 shares of dw
+  float* wl = (float*)ro_lds4;
   float2* trig = (float2*)ro_lds4;
-  __shared__ float red[4][RO_M_MAX];
   const int side = blockIdx.z;
   const RoSide& S = p.s[side];
-  const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR, wave = threadIdx.x >> 6;
-  const RoUnit u = ro_unit<CH, INTER>(p, sub);
+  const RoUnit u = ro_unit<CH, INTER>(p, threadIdx.x % LPR);
   const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
   const unsigned xt = S.x_st * SZ, xh = S.x_sh * SZ, yt = S.y_st * SZ, yh = S.y_sh * SZ, gt = S.g_st * SZ, gh = S.g_sh * SZ;
   float wa[CH], wb[CH], da[CH], db[CH];
+  if ((int)threadIdx.x < p.M) wl[threadIdx.x] = ro_w(S.w, p.w_dtype, threadIdx.x);
+  __syncthreads();
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    wa[c] = ro_w(S.w, p.w_dtype, u.ca + c);
-    wb[c] = ro_w(S.w, p.w_dtype, u.cb + c);
+    wa[c] = wl[u.ca + c];
+    wb[c] = wl[u.cb + c];
     da[c] = db[c] = 0.f;
   }
+  const int run = p.shared ? seg1 - seg0 : 1;
   for (int tile = blockIdx.x; tile < p.ntiles; tile += gridDim.x) {
     const int64_t t0 = (int64_t)tile * p.tile;
-    const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile, items = ntok * S.H;
-    for (int seg = seg0; seg < seg1; ++seg) {
-      if (seg == seg0 || !p.shared) {
-        __syncthreads();                                 // the angles before are no longer read
-        ro_tile_angles(p, trig, seg, t0, ntok);
-        __syncthreads();
-      }
-      const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
-      const char* g = (const char*)S.g + (seg * S.g_sb + t0 * S.g_st) * SZ;
-      char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
-      for (int base = 0; base < items; base += IPT * ROWS) {
-        ro_vec<T, CH> xa[IPT], xb[IPT], ya[IPT], yb[IPT];
-        unsigned yo[IPT];
-        int tok[IPT];
-        bool ok[IPT];
+    const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile;
+    const RoRows<T, CH, LPR, 1> rows = {ntok * S.H, S.H, p.h_magic[side]};
+    for (int first = seg0; first < seg1; first += run) {
+      __syncthreads();                                 // the weights, or the angles before, are no longer read
+      ro_tile_angles(p, trig, first, t0, ntok);
+      __syncthreads();
+      ro_vec<T, CH> xa, xb, ga_, gb_, nxa, nxb, nga, ngb;
+      const auto load = [&](int seg, int base, ro_vec<T, CH>& va, ro_vec<T, CH>& vb, ro_vec<T, CH>& vc, ro_vec<T, CH>& vd) {
+        const char* x = (const char*)S.x + (seg * S.x_sb + t0 * S.x_st) * SZ;
+        const char* g = (const char*)S.g + (seg * S.g_sb + t0 * S.g_st) * SZ;
+        int tt, h;
+        bool ok;
+        rows.at(base, 0, tt, h, ok);
+        const unsigned xo = __umul24(tt, xt) + __umul24(h, xh), go = __umul24(tt, gt) + __umul24(h, gh);
+        va = ro_load<T, CH>(x, xo + u.ca * SZ);
+        vb = ro_load<T, CH>(x, xo + u.cb * SZ);
+        vc = ro_load<T, CH>(g, go + u.ca * SZ);
+        vd = ro_load<T, CH>(g, go + u.cb * SZ);
+      };
+      int seg = first, base = 0;
+      load(seg, 0, xa, xb, ga_, gb_);
+      for (;;) {
+        int nseg = seg, nbase = base + STEP;
+        if (nbase >= rows.items) { nbase = 0; ++nseg; }
+        const bool more = nseg < first + run;
+        if (more) load(nseg, nbase, nxa, nxb, nga, ngb);
+        int tt, h;
+        bool ok;
+        rows.at(base, 0, tt, h, ok);
+        float a[CH], b[CH], ga[CH], gb[CH], s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-          const int idx = base + i * ROWS + slot;
-          ok[i] = idx < items && u.on;
-          const int tt = (int)ro_div(idx, S.H, p.h_magic[side]), h = idx - tt * S.H;
-          tok[i] = tt;
-          yo[i] = __umul24(tt, yt) + __umul24(h, yh);
-          if (ok[i]) {
-            const unsigned xo = __umul24(tt, xt) + __umul24(h, xh), go = __umul24(tt, gt) + __umul24(h, gh);
-            xa[i] = ro_load<T, CH>(x, xo + u.ca * SZ);
-            xb[i] = ro_load<T, CH>(x, xo + u.cb * SZ);
-            ya[i] = ro_load<T, CH>(g, go + u.ca * SZ);
-            yb[i] = ro_load<T, CH>(g, go + u.cb * SZ);
-          }
+        for (int c = 0; c < CH; ++c) {
+          a[c] = (float)xa[c]; b[c] = (float)xb[c];
+          ga[c] = (float)ga_[c]; gb[c] = (float)gb_[c];
         }
+        if (u.turns) ro_turn<CH, INTER>(ga, gb, (const float4*)(trig + tt * p.R + u.j0));
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-          float a[CH], b[CH], ga[CH], gb[CH], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            a[c] = (float)xa[i][c]; b[c] = (float)xb[i][c];
-            ga[c] = (float)ya[i][c]; gb[c] = (float)yb[i][c];
-          }
-          if (u.turns && ok[i]) ro_turn<CH, INTER>(ga, gb, (const float4*)(trig + tok[i] * p.R + u.j0));
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            s1 = fmaf(a[c], a[c], s1); s1 = fmaf(b[c], b[c], s1);
-            s2 = fmaf(ga[c] * wa[c], a[c], s2); s2 = fmaf(gb[c] * wb[c], b[c], s2);
-          }
-          if (LPR > 2 && !u.on) s1 = s2 = 0.f;
-          const float r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s1), p.inv_m, p.eps));
-          const float m = r * r * r * (ro_lane_sum<LPR>(s2) * p.inv_m);
-          if (!ok[i]) continue;
+        for (int c = 0; c < CH; ++c) {
+          s1 = fmaf(a[c], a[c], s1); s1 = fmaf(b[c], b[c], s1);
+          s2 = fmaf(ga[c] * wa[c], a[c], s2); s2 = fmaf(gb[c] * wb[c], b[c], s2);
+        }
+        if (LPR > 2 && !u.on) s1 = s2 = 0.f;
+        const float r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s1), p.inv_m, p.eps));
+        const float m = r * r * r * (ro_lane_sum<LPR>(s2) * p.inv_m);
+        if (ok && u.on) {
+          char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
+          const unsigned yo = __umul24(tt, yt) + __umul24(h, yh);
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             ga[c] *= r; gb[c] *= r;
@@ -442,30 +478,40 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
             a[c] = ga[c] * wa[c] - a[c] * m;
             b[c] = gb[c] * wb[c] - b[c] * m;
           }
-          ro_store<T, CH>(y, yo[i] + u.ca * SZ, a);
-          ro_store<T, CH>(y, yo[i] + u.cb * SZ, b);
+          ro_store<T, CH>(y, yo + u.ca * SZ, a);
+          ro_store<T, CH>(y, yo + u.cb * SZ, b);
         }
+        if (!more) break;
+        xa = nxa; xb = nxb; ga_ = nga; gb_ = ngb;
+        seg = nseg;
+        base = nbase;
       }
     }
   }
   if (!p.parts) return;
+  // rows of 16 lanes by register moves, the 16 rows of the workgroup through LDS (for 32 lanes to a head, two rows hold it)
+  __syncthreads();
+  float* red = (float*)ro_lds4;                        // (shares, M)
+  constexpr int SPAN = LPR < 16 ? 16 : LPR, SHARES = RO_THREADS / SPAN;
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
+  for (int c = 0; c < CH; ++c) { da[c] = ro_row_of_16<LPR>(da[c]); db[c] = ro_row_of_16<LPR>(db[c]); }
+  if ((int)threadIdx.x % SPAN < LPR && u.on)
 #pragma unroll
-    for (int k = LPR; k < 64; k <<= 1) { da[c] += __shfl_xor(da[c], k, 64); db[c] += __shfl_xor(db[c], k, 64); }
-    if ((threadIdx.x & 63) < LPR && u.on) { red[wave][u.ca + c] = da[c]; red[wave][u.cb + c] = db[c]; }
-  }
+    for (int c = 0; c < CH; ++c) {
+      red[threadIdx.x / SPAN * p.M + u.ca + c] = da[c];
+      red[threadIdx.x / SPAN * p.M + u.cb + c] = db[c];
+    }
   __syncthreads();
   const int64_t row = (int64_t)side * p.nblocks + blockIdx.y * gridDim.x + blockIdx.x;
-  for (int c = threadIdx.x; c < p.M; c += RO_THREADS)
-    p.parts[row * p.M + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  if ((int)threadIdx.x < p.M) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < SHARES; ++i) s += red[i * p.M + threadIdx.x];
+    p.parts[row * p.M + threadIdx.x] = s;
+  }
 }
 
-unsigned ro_magic(int64_t most, int64_t d) {           // x / d == umulhi(x, magic) for every x <= most, else 0
-  const uint64_t m = ((1ull << 32) + (uint64_t)d - 1) / (uint64_t)d;
-  if (d < 2 || m >= (1ull << 32) || most >= (1ll << 32)) return 0;
-  return (m * (uint64_t)d - (1ull << 32)) * (uint64_t)most < (1ull << 32) ? (unsigned)m : 0u;
-}
+unsigned ro_magic(int d) { return (unsigned)(((1ull << 31) + d - 1) / d); }
 
 // Channels of a chunk: 16 bytes where the head, the rotated part and every stride and address allow it, else 8 bytes of a 16-bit
 // type, else 0: one element at a time (as where a token or head stride passes the 24 bits of a factor).
@@ -493,9 +539,10 @@ int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
   return 0;
 }
 
-// Tiles and segments of a launch: `rows` head rows of one side to a workgroup at the most, angles in 16 KB, and at least `want`
-// workgroups where there is work for them.
-void ro_plan(RoParams& p, int size, int rows, int64_t want) {
+// Tiles and segments of a launch: a tile's rows fill whole steps of the workgroup (`step` head rows; up to four), its angles 16 KB
+// at the most, and there are `want` workgroups where there is work for them: as many as the device holds at once, of equal
+// work, so that none is left for a second round.
+void ro_plan(RoParams& p, int size, int step, int64_t want) {
   bool flat = true;                                    // images follow each other in every tensor
   int64_t st = 1;
   for (int i = 0; i < p.sides; ++i) {
@@ -505,12 +552,14 @@ void ro_plan(RoParams& p, int size, int rows, int64_t want) {
   }
   const bool shared = p.R == 0 || p.pos_sb == 0 || p.B == 1;
   const int H = p.s[0].H > p.s[1].H ? p.s[0].H : p.s[1].H;
-  int64_t tile = rows / H;
-  if (tile > 512) tile = 512;
+  const int64_t tokens = (int64_t)p.B * p.N;
+  int64_t tile = 512;
   if (p.R > 0 && tile > 2048 / p.R) tile = 2048 / p.R;
   if (tile > (1 << 30) / (st * size)) tile = (1 << 30) / (st * size);
-  const int64_t tokens = (int64_t)p.B * p.N;
   if (tile > (tokens + want - 1) / want) tile = (tokens + want - 1) / want;
+  int64_t steps = tile * H / step;
+  if (steps > 4) steps = 4;
+  if (steps >= 1) tile = steps * step / H;
   if (tile < 1) tile = 1;
   // one segment of all tokens for positions of each image's own, and for images shorter than a tile
   p.flat = flat && p.B > 1 && (!shared || p.N < tile);
@@ -522,17 +571,17 @@ void ro_plan(RoParams& p, int size, int rows, int64_t want) {
   p.spg = 1;
   p.shared = shared;
   if (shared && p.nseg > 1) {
-    const int64_t units = (int64_t)p.ntiles * p.nseg, spg = units / want;
-    p.spg = spg < 1 ? 1 : spg > p.nseg ? p.nseg : (int)spg;
+    const int64_t units = (int64_t)p.ntiles * p.nseg, spg = (units + want - 1) / want;
+    p.spg = spg > p.nseg ? p.nseg : (int)spg;
   }
-  for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic((int64_t)p.tile * p.s[i].H + 2 * RO_THREADS, p.s[i].H);
-  p.n_magic = ro_magic((int64_t)p.N + p.tile, p.N);
-  p.r_magic = p.R ? ro_magic((int64_t)p.tile * p.R, p.R) : 0;
+  for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic(p.s[i].H);      // rows of a tile <= 2^16, heads < 2^7
+  p.n_magic = p.flat && p.N < p.tile ? ro_magic(p.N) : 0;                   // both <= 2^9
+  p.r_magic = p.R ? ro_magic(p.R) : 0;                                      // angles <= 2^11 or pairs of one token
 }
 
 template <typename T, int CH, int LPR, bool NORM>
 int ro_tile_launch(RoParams& p, hipStream_t s) {
-  ro_plan(p, sizeof(T), 4 * RO_THREADS / LPR, 1536);
+  ro_plan(p, sizeof(T), 2 * RO_THREADS / LPR, (NORM ? 5 : 6) * vil_cu_count());
   if (p.nseg > 65535 * (int64_t)p.spg) p.spg = (p.nseg + 65534) / 65535;         // (the grid's second axis)
   const dim3 grid(p.ntiles, (p.nseg + p.spg - 1) / p.spg), block(RO_THREADS);
   const size_t lds = (size_t)p.tile * p.R * sizeof(float2) + (NORM ? 2 * p.M * sizeof(float) : 0);
@@ -543,12 +592,13 @@ int ro_tile_launch(RoParams& p, hipStream_t s) {
 
 template <typename T, int CH, int LPR>
 int ro_bwd_launch(RoParams& p, hipStream_t s) {
-  ro_plan(p, sizeof(T), 4 * RO_THREADS / LPR, RO_BWD_BLOCKS);
+  const int held = 4 * vil_cu_count() / p.sides;
+  ro_plan(p, sizeof(T), RO_THREADS / LPR, held < RO_BWD_BLOCKS ? held : RO_BWD_BLOCKS);
   if (p.nseg > RO_BWD_BLOCKS * (int64_t)p.spg) p.spg = (p.nseg + RO_BWD_BLOCKS - 1) / RO_BWD_BLOCKS;   // (short images)
   const int groups = (p.nseg + p.spg - 1) / p.spg, x = RO_BWD_BLOCKS / groups;
   const dim3 grid(x < p.ntiles ? x : p.ntiles, groups, p.sides), block(RO_THREADS);
   p.nblocks = grid.x * grid.y;
-  const size_t lds = (size_t)p.tile * p.R * sizeof(float2);
+  const size_t angles = (size_t)p.tile * p.R * sizeof(float2), shares = (size_t)16 * p.M * sizeof(float), lds = angles > shares ? angles : shares;
   if (p.interleaved) k_rope_norm_bwd<T, CH, LPR, true><<<grid, block, lds, s>>>(p);
   else k_rope_norm_bwd<T, CH, LPR, false><<<grid, block, lds, s>>>(p);
   return (int)hipGetLastError();
