@@ -216,6 +216,8 @@ constexpr int RO_BWD_BLOCKS = 1024;                    // workgroups of one side
 // angles of a token are taken once, into LDS, and serve every head of q and k.  Segments are the images; where all share
 // their positions a workgroup walks several of them with the same angles.  Where a tensor's images follow each other
 // (stride of an image = N tokens) and positions are each image's own, all tokens are one segment, so that short images fill a tile.
+// A workgroup's segments lie gridDim.y apart: the workgroups of a moment read one window of the tensors, in order (their own
+// consecutive segments each: 8 % slower).
 // Addresses: a scalar base per segment and 32-bit byte offsets inside the tile (products of 24-bit factors).
 template <typename T, int CH> using ro_vec = T __attribute__((ext_vector_type(CH)));
 
@@ -290,7 +292,7 @@ template <typename T, int CH> __device__ __forceinline__ void ro_store(char* bas
   ro_vec<T, CH> o;
 #pragma unroll
   for (int c = 0; c < CH; ++c) o[c] = (T)v[c];
-  *(ro_vec<T, CH>*)(base + off) = o;
+  __builtin_nontemporal_store(o, (ro_vec<T, CH>*)(base + off));   // (streams past the caches: 10 to 15 % of the large cases' time)
 }
 
 // Head rows of a tile, one side: IPT rows to a thread and step, the next step's loads issued before this one's arithmetic, so that
@@ -318,13 +320,13 @@ __global__ __launch_bounds__(RO_THREADS, NORM ? 4 : 5) void k_rope_tile(RoParams
   float2* trig = (float2*)(wl + (NORM ? 2 * p.M : 0));
   const int64_t t0 = (int64_t)blockIdx.x * p.tile;
   const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile;
-  const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
   const RoUnit u = ro_unit<CH, INTER>(p, threadIdx.x % LPR);
   if (NORM)
     for (int c = threadIdx.x; c < 2 * p.M; c += RO_THREADS) wl[c] = c < p.M ? ro_w(p.s[0].w, p.w_dtype, c) : ro_w(p.s[1].w, p.w_dtype, c - p.M);
-  const int run = p.shared ? seg1 - seg0 : 1;                    // segments that the same angles serve
-  for (int first = seg0; first < seg1; first += run) {
-    if (first != seg0) __syncthreads();                          // the angles before are no longer read
+  const int stride = gridDim.y;
+  for (int first = blockIdx.y; first < p.nseg; first += stride) {
+    const int last = p.shared ? p.nseg : first + 1;              // segments that the same angles serve
+    if (first != (int)blockIdx.y) __syncthreads();               // the angles before are no longer read
     ro_tile_angles(p, trig, first, t0, ntok);
     __syncthreads();
     for (int side = 0; side < p.sides; ++side) {
@@ -352,8 +354,8 @@ __global__ __launch_bounds__(RO_THREADS, NORM ? 4 : 5) void k_rope_tile(RoParams
       load(seg, 0, xa, xb);
       for (;;) {
         int nseg = seg, nbase = base + STEP;
-        if (nbase >= rows.items) { nbase = 0; ++nseg; }
-        const bool more = nseg < first + run;
+        if (nbase >= rows.items) { nbase = 0; nseg += stride; }
+        const bool more = nseg < last;
         if (more) load(nseg, nbase, na, nb);
         char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
 #pragma unroll
@@ -387,6 +389,7 @@ __global__ __launch_bounds__(RO_THREADS, NORM ? 4 : 5) void k_rope_tile(RoParams
         base = nbase;
       }
     }
+    if (p.shared) break;
   }
 }
 
@@ -409,7 +412,6 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
   const int side = blockIdx.z;
   const RoSide& S = p.s[side];
   const RoUnit u = ro_unit<CH, INTER>(p, threadIdx.x % LPR);
-  const int seg0 = blockIdx.y * p.spg, seg1 = seg0 + p.spg < p.nseg ? seg0 + p.spg : p.nseg;
   const unsigned xt = S.x_st * SZ, xh = S.x_sh * SZ, yt = S.y_st * SZ, yh = S.y_sh * SZ, gt = S.g_st * SZ, gh = S.g_sh * SZ;
   float wa[CH], wb[CH], da[CH], db[CH];
   if ((int)threadIdx.x < p.M) wl[threadIdx.x] = ro_w(S.w, p.w_dtype, threadIdx.x);
@@ -420,12 +422,13 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
     wb[c] = wl[u.cb + c];
     da[c] = db[c] = 0.f;
   }
-  const int run = p.shared ? seg1 - seg0 : 1;
+  const int stride = gridDim.y;
   for (int tile = blockIdx.x; tile < p.ntiles; tile += gridDim.x) {
     const int64_t t0 = (int64_t)tile * p.tile;
     const int ntok = p.T - t0 < p.tile ? (int)(p.T - t0) : p.tile;
     const RoRows<T, CH, LPR, 1> rows = {ntok * S.H, S.H, p.h_magic[side]};
-    for (int first = seg0; first < seg1; first += run) {
+    for (int first = blockIdx.y; first < p.nseg; first += stride) {
+      const int last = p.shared ? p.nseg : first + 1;
       __syncthreads();                                 // the weights, or the angles before, are no longer read
       ro_tile_angles(p, trig, first, t0, ntok);
       __syncthreads();
@@ -446,8 +449,8 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
       load(seg, 0, xa, xb, ga_, gb_);
       for (;;) {
         int nseg = seg, nbase = base + STEP;
-        if (nbase >= rows.items) { nbase = 0; ++nseg; }
-        const bool more = nseg < first + run;
+        if (nbase >= rows.items) { nbase = 0; nseg += stride; }
+        const bool more = nseg < last;
         if (more) load(nseg, nbase, nxa, nxb, nga, ngb);
         int tt, h;
         bool ok;
@@ -486,6 +489,7 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
         seg = nseg;
         base = nbase;
       }
+      if (p.shared) break;
     }
   }
   if (!p.parts) return;
@@ -540,9 +544,10 @@ int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
 }
 
 // Tiles and segments of a launch: a tile's rows fill whole steps of the workgroup (`step` head rows; up to four), its angles 16 KB
-// at the most, and there are `want` workgroups where there is work for them: as many as the device holds at once, of equal
-// work, so that none is left for a second round.
-void ro_plan(RoParams& p, int size, int step, int64_t want) {
+// at the most (32 KB: 15 % slower), and there are at least `want` workgroups where there is work for them.  Segments that share their
+// angles are walked by one workgroup only past `rounds` times `want` of them: the forward pass at 32 x 9217 x 3 heads of 32 takes
+// 50 us with a workgroup to each of 3488 tiles, 54 with 1744, 57 with 1163.
+void ro_plan(RoParams& p, int size, int step, int64_t want, int rounds) {
   bool flat = true;                                    // images follow each other in every tensor
   int64_t st = 1;
   for (int i = 0; i < p.sides; ++i) {
@@ -571,7 +576,7 @@ void ro_plan(RoParams& p, int size, int step, int64_t want) {
   p.spg = 1;
   p.shared = shared;
   if (shared && p.nseg > 1) {
-    const int64_t units = (int64_t)p.ntiles * p.nseg, spg = (units + want - 1) / want;
+    const int64_t units = (int64_t)p.ntiles * p.nseg, most = want * rounds, spg = (units + most - 1) / most;
     p.spg = spg > p.nseg ? p.nseg : (int)spg;
   }
   for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic(p.s[i].H);      // rows of a tile <= 2^16, heads < 2^7
@@ -581,7 +586,7 @@ void ro_plan(RoParams& p, int size, int step, int64_t want) {
 
 template <typename T, int CH, int LPR, bool NORM>
 int ro_tile_launch(RoParams& p, hipStream_t s) {
-  ro_plan(p, sizeof(T), 2 * RO_THREADS / LPR, (NORM ? 5 : 6) * vil_cu_count());
+  ro_plan(p, sizeof(T), 2 * RO_THREADS / LPR, 5 * vil_cu_count(), 8);
   if (p.nseg > 65535 * (int64_t)p.spg) p.spg = (p.nseg + 65534) / 65535;         // (the grid's second axis)
   const dim3 grid(p.ntiles, (p.nseg + p.spg - 1) / p.spg), block(RO_THREADS);
   const size_t lds = (size_t)p.tile * p.R * sizeof(float2) + (NORM ? 2 * p.M * sizeof(float) : 0);
@@ -592,8 +597,9 @@ int ro_tile_launch(RoParams& p, hipStream_t s) {
 
 template <typename T, int CH, int LPR>
 int ro_bwd_launch(RoParams& p, hipStream_t s) {
-  const int held = 4 * vil_cu_count() / p.sides;
-  ro_plan(p, sizeof(T), RO_THREADS / LPR, held < RO_BWD_BLOCKS ? held : RO_BWD_BLOCKS);
+  // two workgroups to a CU: every one ends in a row of partial sums (four: 7 % slower at 128 x 3137 x 3 heads of 32, one: 14 %)
+  const int held = 2 * vil_cu_count() / p.sides;
+  ro_plan(p, sizeof(T), RO_THREADS / LPR, held < RO_BWD_BLOCKS ? held : RO_BWD_BLOCKS, 1);
   if (p.nseg > RO_BWD_BLOCKS * (int64_t)p.spg) p.spg = (p.nseg + RO_BWD_BLOCKS - 1) / RO_BWD_BLOCKS;   // (short images)
   const int groups = (p.nseg + p.spg - 1) / p.spg, x = RO_BWD_BLOCKS / groups;
   const dim3 grid(x < p.ntiles ? x : p.ntiles, groups, p.sides), block(RO_THREADS);
