@@ -547,7 +547,7 @@ int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
 // at the most (32 KB: 15 % slower), and there are at least `want` workgroups where there is work for them.  Segments that share their
 // angles are walked by one workgroup only past `rounds` times `want` of them: the forward pass at 32 x 9217 x 3 heads of 32 takes
 // 50 us with a workgroup to each of 3488 tiles, 54 with 1744, 57 with 1163.
-void ro_plan(RoParams& p, int size, int step, int64_t want, int rounds) {
+void ro_plan(RoParams& p, int size, int wave_rows, int step, int64_t want, int rounds) {
   bool flat = true;                                    // images follow each other in every tensor
   int64_t st = 1;
   for (int i = 0; i < p.sides; ++i) {
@@ -561,7 +561,8 @@ void ro_plan(RoParams& p, int size, int step, int64_t want, int rounds) {
   int64_t tile = 512;
   if (p.R > 0 && tile > 2048 / p.R) tile = 2048 / p.R;
   if (tile > (1 << 30) / (st * size)) tile = (1 << 30) / (st * size);
-  if (tile > (tokens + want - 1) / want) tile = (tokens + want - 1) / want;
+  const int64_t share = (tokens + want - 1) / want, wave = (wave_rows + H - 1) / H;      // (a wave's worth of rows at least)
+  if (tile > (share > wave ? share : wave)) tile = share > wave ? share : wave;
   int64_t steps = tile * H / step;
   if (steps > 4) steps = 4;
   if (steps >= 1) tile = steps * step / H;
@@ -586,7 +587,7 @@ void ro_plan(RoParams& p, int size, int step, int64_t want, int rounds) {
 
 template <typename T, int CH, int LPR, bool NORM>
 int ro_tile_launch(RoParams& p, hipStream_t s) {
-  ro_plan(p, sizeof(T), 2 * RO_THREADS / LPR, 5 * vil_cu_count(), 8);
+  ro_plan(p, sizeof(T), 64 / LPR, 2 * RO_THREADS / LPR, 5 * vil_cu_count(), 8);
   if (p.nseg > 65535 * (int64_t)p.spg) p.spg = (p.nseg + 65534) / 65535;         // (the grid's second axis)
   const dim3 grid(p.ntiles, (p.nseg + p.spg - 1) / p.spg), block(RO_THREADS);
   const size_t lds = (size_t)p.tile * p.R * sizeof(float2) + (NORM ? 2 * p.M * sizeof(float) : 0);
@@ -599,7 +600,7 @@ template <typename T, int CH, int LPR>
 int ro_bwd_launch(RoParams& p, hipStream_t s) {
   // two workgroups to a CU: every one ends in a row of partial sums (four: 7 % slower at 128 x 3137 x 3 heads of 32, one: 14 %)
   const int held = 2 * vil_cu_count() / p.sides;
-  ro_plan(p, sizeof(T), RO_THREADS / LPR, held < RO_BWD_BLOCKS ? held : RO_BWD_BLOCKS, 1);
+  ro_plan(p, sizeof(T), 64 / LPR, RO_THREADS / LPR, held < RO_BWD_BLOCKS ? held : RO_BWD_BLOCKS, 1);
   if (p.nseg > RO_BWD_BLOCKS * (int64_t)p.spg) p.spg = (p.nseg + RO_BWD_BLOCKS - 1) / RO_BWD_BLOCKS;   // (short images)
   const int groups = (p.nseg + p.spg - 1) / p.spg, x = RO_BWD_BLOCKS / groups;
   const dim3 grid(x < p.ntiles ? x : p.ntiles, groups, p.sides), block(RO_THREADS);
