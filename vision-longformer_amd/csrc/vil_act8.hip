@@ -74,80 +74,237 @@ __device__ __forceinline__ float a8_slope(float g, float x, float hx, float s) {
   return x < 0.f ? u * s : fmaf(-u, s, g);
 }
 
-// One block of 32 channels to 32 lanes, one value to a lane.  GELU: a = gelu(x) beside the packed x.
-template <typename T, bool GELU>
-__global__ __launch_bounds__(256) void k_act8_pack(const T* x, int64_t x_rs, int64_t rows, int cols, T* a, int8_t* codes, uint8_t* scales) {
-  const int nb = (cols + A8_BLOCK - 1) / A8_BLOCK;
-  const int64_t blk = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t row = blk / nb;
-  const int ib = (int)(blk - row * nb), c = ib * A8_BLOCK + (threadIdx.x & 31);
-  const bool ok = row < rows && c < cols;
-  const float v = ok ? (float)x[row * x_rs + c] : 0.f;
-  uint32_t m = __float_as_uint(v) & 0x7fffffffu;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint32_t other = __shfl_xor(m, o, 32);
-    m = other > m ? other : m;
+// Eight neighbouring channels to a lane, four lanes to a block of 32: one 16-byte load of a 16-bit type, and a block's maximum in two
+// register moves.  A workgroup takes A8_CHUNKS chunks of 256 lanes, all loads first.  FLAT: rows without gaps whose channels fill
+// their blocks are one long row.  Otherwise a lane finds its row by a division; rows need no alignment (the memory system takes
+// 16 bytes at any address of the type), and only a row's last lane goes value by value.
+constexpr int A8_THREADS = 256, A8_CHUNKS = 2;
+template <typename T> using a8_vec = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+template <typename T> using a8_vec16 = T __attribute__((ext_vector_type(8)));
+typedef unsigned a8_codes __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned a8_codes8 __attribute__((ext_vector_type(2)));
+
+struct A8At { int64_t row, blk; int c, n; };               // row, block, first channel, channels of this lane (0: none)
+template <bool FLAT>
+__device__ __forceinline__ A8At a8_at(int64_t lane, int64_t rows, int cols, int nb) {
+  A8At w;
+  w.blk = lane >> 2;
+  if (FLAT) {                                              // (cols: of the one row; 64-bit offsets in `row`)
+    w.row = lane * 8;
+    w.c = 0;
+    w.n = w.row < rows ? 8 : 0;                            // (rows: the number of values)
+    return w;
   }
-  const int e = a8_exponent(m);
-  if (!ok) return;
-  float r = e == 255 ? 0.f : rintf(v * a8_inverse(e));
-  if (e == A8Top<T>::biased) r = fminf(fmaxf(r, -63.f), 63.f);
-  codes[row * cols + c] = (int8_t)(int)r;
-  if ((threadIdx.x & 31) == 0) scales[blk] = (uint8_t)e;
-  if (GELU) {
-    float hx, s;
-    a8_gelu<sizeof(T) == 4>(v, hx, s);
-    a[row * cols + c] = (T)(v == INFINITY ? v : a8_act(v, hx, s));
+  if (rows * nb < ((int64_t)1 << 31)) w.row = (uint32_t)w.blk / (uint32_t)nb;
+  else w.row = w.blk / nb;
+  w.c = (int)(w.blk - w.row * nb) * A8_BLOCK + (int)(lane & 3) * 8;
+  w.n = w.row < rows ? cols - w.c : 0;
+  w.n = w.n < 0 ? 0 : w.n > 8 ? 8 : w.n;
+  return w;
+}
+
+template <typename T, bool FLAT> __device__ __forceinline__ a8_vec16<T> a8_load(const T* p, int n) {
+  if (FLAT) return n ? *(const a8_vec16<T>*)p : (a8_vec16<T>)(T)0;
+  if (n == 8) return *(const a8_vec<T>*)p;
+  a8_vec16<T> v = (a8_vec16<T>)(T)0;
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < n) v[i] = p[i];
+  return v;
+}
+template <typename T, bool FLAT> __device__ __forceinline__ void a8_store(T* p, const float (&v)[8], int n) {
+  a8_vec16<T> o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = (T)v[i];
+  if (FLAT) { if (n) *(a8_vec16<T>*)p = o; return; }
+  if (n == 8) { *(a8_vec<T>*)p = o; return; }
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < n) p[i] = o[i];
+}
+
+// the bits of the largest |x| of a lane, as fp32 bits: the types' bits without the sign order as the magnitudes do, NaN last
+template <typename T> __device__ __forceinline__ uint32_t a8_lane_max(const a8_vec16<T>& x) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+    return m;
+  } else {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    const u4 w = __builtin_bit_cast(u4, x) & 0x7fff7fffu;
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];             // (a bit cast of a vector's element reads its first)
+    const us2 m = __builtin_elementwise_max(__builtin_elementwise_max(__builtin_bit_cast(us2, w0), __builtin_bit_cast(us2, w1)),
+                                            __builtin_elementwise_max(__builtin_bit_cast(us2, w2), __builtin_bit_cast(us2, w3)));
+    const unsigned short h = m[0] > m[1] ? m[0] : m[1];
+    return __float_as_uint((float)__builtin_bit_cast(T, h));
+  }
+}
+template <int CTRL> __device__ __forceinline__ uint32_t a8_quad(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+  return o > v ? o : v;
+}
+
+// GELU: a = gelu(x) beside the packed x
+template <typename T, bool GELU, bool FLAT>
+__global__ __launch_bounds__(A8_THREADS) void k_act8_pack(const T* x, int64_t x_rs, int64_t rows, int cols, int nb, T* a, int8_t* codes,
+                                                           uint8_t* scales) {
+  const int64_t lane0 = (int64_t)blockIdx.x * (A8_THREADS * A8_CHUNKS) + threadIdx.x;
+  a8_vec16<T> in[A8_CHUNKS];
+  A8At at[A8_CHUNKS];
+#pragma unroll
+  for (int k = 0; k < A8_CHUNKS; ++k) {
+    at[k] = a8_at<FLAT>(lane0 + k * A8_THREADS, rows, cols, nb);
+    in[k] = a8_load<T, FLAT>(x + (FLAT ? at[k].row : at[k].row * x_rs + at[k].c), at[k].n);
+  }
+#pragma unroll
+  for (int k = 0; k < A8_CHUNKS; ++k) {
+    const A8At& w = at[k];
+    const int e = a8_exponent(a8_quad<0x4e>(a8_quad<0xb1>(a8_lane_max<T>(in[k]))));
+    const float inv = a8_inverse(e == 255 ? 1 : e);
+    float v[8];
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = (float)in[k][i];
+      c[i] = __float_as_uint(fmaf(v[i], inv, 12582912.f));                 // 1.5 * 2^23: the sum's last byte is the rounded integer
+    }
+    if (e >= A8Top<T>::biased) {                                           // (rare: the type's largest numbers, or a marked block)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = e == 255 ? 0u : (uint32_t)(int)fminf(fmaxf(rintf(v[i] * inv), -63.f), 63.f);
+    }
+    a8_codes8 o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0c0c0400u);
+      o[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    }
+    if (!w.n) continue;
+    const int64_t to = FLAT ? w.row : w.row * cols + w.c;
+    if (FLAT) *(a8_codes8*)(codes + to) = o;
+    else if (w.n == 8) *(a8_codes*)(codes + to) = o;
+    else
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < w.n) codes[to + i] = (int8_t)c[i];
+    if ((threadIdx.x & 3) == 0) scales[w.blk] = (uint8_t)e;
+    if (GELU) {
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float hx, s;
+        a8_gelu<sizeof(T) == 4>(v[i], hx, s);
+        r[i] = a8_act(v[i], hx, s);
+      }
+      if (e == 255)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = v[i] == INFINITY ? v[i] : r[i];
+      a8_store<T, FLAT>(a + to, r, w.n);
+    }
   }
 }
 
 // values from codes; GELU: dh = da * gelu'(value) and, where `a` is wanted, gelu(value)
-template <typename T, bool GELU>
-__global__ __launch_bounds__(256) void k_act8_unpack(const int8_t* codes, const uint8_t* scales, const T* da, int64_t da_rs,
-                                                     int64_t rows, int cols, T* out, T* a) {
-  const int nb = (cols + A8_BLOCK - 1) / A8_BLOCK;
-  const int64_t blk = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t row = blk / nb;
-  const int ib = (int)(blk - row * nb), c = ib * A8_BLOCK + (threadIdx.x & 31);
-  if (row >= rows || c >= cols) return;
-  const int e = scales[blk];
-  const float v = e == 255 ? __uint_as_float(0x7fc00000u) : (float)codes[row * cols + c] * a8_pow2(e);
-  if (!GELU) { out[row * cols + c] = (T)v; return; }
-  float hx, s;
-  a8_gelu<sizeof(T) == 4>(v, hx, s);
-  out[row * cols + c] = (T)a8_slope((float)da[row * da_rs + c], v, hx, s);
-  if (a) a[row * cols + c] = (T)a8_act(v, hx, s);
+template <typename T, bool GELU, bool FLAT>
+__global__ __launch_bounds__(A8_THREADS) void k_act8_unpack(const int8_t* codes, const uint8_t* scales, const T* da, int64_t da_rs,
+                                                            int64_t rows, int cols, int nb, T* out, T* a) {
+  const int64_t lane0 = (int64_t)blockIdx.x * (A8_THREADS * A8_CHUNKS) + threadIdx.x;
+  a8_codes8 in[A8_CHUNKS];
+  a8_vec16<T> g[A8_CHUNKS];
+  int e[A8_CHUNKS];
+  A8At at[A8_CHUNKS];
+#pragma unroll
+  for (int k = 0; k < A8_CHUNKS; ++k) {
+    const A8At w = at[k] = a8_at<FLAT>(lane0 + k * A8_THREADS, rows, cols, nb);
+    const int8_t* from = codes + (FLAT ? w.row : w.row * cols + w.c);
+    in[k] = (a8_codes8)0u;
+    e[k] = 1;
+    if (FLAT) { if (w.n) in[k] = *(const a8_codes8*)from; }
+    else if (w.n == 8) in[k] = *(const a8_codes*)from;
+    else
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < w.n) in[k][i / 4] |= (uint32_t)(uint8_t)from[i] << (8 * (i % 4));
+    if (w.n) e[k] = scales[w.blk];
+    if (GELU) g[k] = a8_load<T, FLAT>(da + (FLAT ? w.row : w.row * da_rs + w.c), w.n);
+  }
+#pragma unroll
+  for (int k = 0; k < A8_CHUNKS; ++k) {
+    const A8At& w = at[k];
+    const float step = e[k] == 255 ? __uint_as_float(0x7fc00000u) : a8_pow2(e[k]);
+    const int64_t to = FLAT ? w.row : w.row * cols + w.c;
+    float v[8], r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)(int)(int8_t)(in[k][i / 4] >> (8 * (i % 4))) * step;
+    if (GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float hx, s;
+        a8_gelu<sizeof(T) == 4>(v[i], hx, s);
+        r[i] = a8_slope((float)g[k][i], v[i], hx, s);
+        v[i] = a8_act(v[i], hx, s);
+      }
+      a8_store<T, FLAT>(out + to, r, w.n);
+      if (a) a8_store<T, FLAT>(a + to, v, w.n);
+    } else {
+      a8_store<T, FLAT>(out + to, v, w.n);
+    }
+  }
 }
 
 int a8_check(int dtype, int64_t rows, int cols, int64_t rs) {
   if (dtype != VIL_DTYPE_F32 && dtype != VIL_DTYPE_BF16 && dtype != VIL_DTYPE_F16) return VIL_E_DTYPE;
   if (rows < 0 || cols < 0 || (rows > 1 && rs < cols)) return VIL_E_SHAPE;
-  // (one workgroup to 256 values at the most: the grid's first axis holds 2^31 - 1)
+  // (a block of 32, filled or not, is four lanes: 2^31 workgroups of 512 lanes hold more than 2^37 values)
   if (cols > 0 && rows > ((int64_t)1 << 37) / cols) return VIL_E_SHAPE;
   return VIL_OK;
 }
-unsigned a8_grid(int64_t rows, int cols) { return (unsigned)((rows * ((cols + A8_BLOCK - 1) / A8_BLOCK) + 7) / 8); }
-
-template <bool GELU>
-int a8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t rs, void* a, void* codes, void* scales, hipStream_t s) {
-  const dim3 grid(a8_grid(rows, cols)), block(256);
-  if (dtype == VIL_DTYPE_F32) k_act8_pack<float, GELU><<<grid, block, 0, s>>>((const float*)x, rs, rows, cols, (float*)a, (int8_t*)codes, (uint8_t*)scales);
-  else if (dtype == VIL_DTYPE_BF16) k_act8_pack<__bf16, GELU><<<grid, block, 0, s>>>((const __bf16*)x, rs, rows, cols, (__bf16*)a, (int8_t*)codes, (uint8_t*)scales);
-  else k_act8_pack<_Float16, GELU><<<grid, block, 0, s>>>((const _Float16*)x, rs, rows, cols, (_Float16*)a, (int8_t*)codes, (uint8_t*)scales);
-  return (int)hipGetLastError();
+// FLAT: rows of whole blocks without gaps, at addresses that the widest access fits; `rows` is then the number of values
+struct A8Shape { int64_t rows; int cols, nb; bool flat; unsigned grid; };
+A8Shape a8_shape(int64_t rows, int cols, int64_t rs, uintptr_t addresses) {
+  A8Shape w;
+  w.nb = (cols + A8_BLOCK - 1) / A8_BLOCK;
+  w.cols = cols;
+  w.flat = cols % A8_BLOCK == 0 && (rs == cols || rows == 1) && addresses % 16 == 0;
+  const int64_t lanes = rows * w.nb * 4, per = A8_THREADS * A8_CHUNKS;
+  w.rows = w.flat ? rows * cols : rows;
+  w.grid = (unsigned)((lanes + per - 1) / per);
+  return w;
 }
 
+template <typename T, bool GELU>
+int a8_pack_t(const void* x, int64_t rows, int cols, int64_t rs, void* a, void* codes, void* scales, hipStream_t s) {
+  const A8Shape w = a8_shape(rows, cols, rs, (uintptr_t)x | (uintptr_t)a | (uintptr_t)codes);
+  if (w.flat) k_act8_pack<T, GELU, true><<<dim3(w.grid), dim3(A8_THREADS), 0, s>>>((const T*)x, rs, w.rows, w.cols, w.nb, (T*)a, (int8_t*)codes, (uint8_t*)scales);
+  else k_act8_pack<T, GELU, false><<<dim3(w.grid), dim3(A8_THREADS), 0, s>>>((const T*)x, rs, w.rows, w.cols, w.nb, (T*)a, (int8_t*)codes, (uint8_t*)scales);
+  return (int)hipGetLastError();
+}
+template <bool GELU>
+int a8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t rs, void* a, void* codes, void* scales, hipStream_t s) {
+  if (dtype == VIL_DTYPE_F32) return a8_pack_t<float, GELU>(x, rows, cols, rs, a, codes, scales, s);
+  if (dtype == VIL_DTYPE_BF16) return a8_pack_t<__bf16, GELU>(x, rows, cols, rs, a, codes, scales, s);
+  return a8_pack_t<_Float16, GELU>(x, rows, cols, rs, a, codes, scales, s);
+}
+
+template <typename T, bool GELU>
+int a8_unpack_t(const void* codes, const void* scales, const void* da, int64_t da_rs, int64_t rows, int cols, void* out, void* a, hipStream_t s) {
+  const A8Shape w = a8_shape(rows, cols, GELU ? da_rs : cols, (uintptr_t)codes | (uintptr_t)da | (uintptr_t)out | (uintptr_t)a);
+  const int8_t* c = (const int8_t*)codes;
+  const uint8_t* e = (const uint8_t*)scales;
+  if (w.flat) k_act8_unpack<T, GELU, true><<<dim3(w.grid), dim3(A8_THREADS), 0, s>>>(c, e, (const T*)da, da_rs, w.rows, w.cols, w.nb, (T*)out, (T*)a);
+  else k_act8_unpack<T, GELU, false><<<dim3(w.grid), dim3(A8_THREADS), 0, s>>>(c, e, (const T*)da, da_rs, w.rows, w.cols, w.nb, (T*)out, (T*)a);
+  return (int)hipGetLastError();
+}
 template <bool GELU>
 int a8_unpack(const void* codes, const void* scales, const void* da, int64_t da_rs, int dtype, int64_t rows, int cols, void* out,
               void* a, hipStream_t s) {
-  const dim3 grid(a8_grid(rows, cols)), block(256);
-  const int8_t* c = (const int8_t*)codes;
-  const uint8_t* e = (const uint8_t*)scales;
-  if (dtype == VIL_DTYPE_F32) k_act8_unpack<float, GELU><<<grid, block, 0, s>>>(c, e, (const float*)da, da_rs, rows, cols, (float*)out, (float*)a);
-  else if (dtype == VIL_DTYPE_BF16) k_act8_unpack<__bf16, GELU><<<grid, block, 0, s>>>(c, e, (const __bf16*)da, da_rs, rows, cols, (__bf16*)out, (__bf16*)a);
-  else k_act8_unpack<_Float16, GELU><<<grid, block, 0, s>>>(c, e, (const _Float16*)da, da_rs, rows, cols, (_Float16*)out, (_Float16*)a);
-  return (int)hipGetLastError();
+  if (dtype == VIL_DTYPE_F32) return a8_unpack_t<float, GELU>(codes, scales, da, da_rs, rows, cols, out, a, s);
+  if (dtype == VIL_DTYPE_BF16) return a8_unpack_t<__bf16, GELU>(codes, scales, da, da_rs, rows, cols, out, a, s);
+  return a8_unpack_t<_Float16, GELU>(codes, scales, da, da_rs, rows, cols, out, a, s);
 }
 
 }  // namespace
