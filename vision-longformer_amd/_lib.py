@@ -268,6 +268,18 @@ def check(code):
         raise VilAttnError(code, lib().vil_attn_strerror(code).decode())
 
 
+def launch(index, fn, *args):
+    """fn(*args, stream) on device `index` and its current stream.  The two torch._C calls are what torch.cuda.current_device() and
+    current_stream() end in, without the objects around them (8 of the 25 microseconds that a small call took)."""
+    if torch._C._cuda_getDevice() == index:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != 0:
+        check(code)
+
+
 def profile_begin(capacity=8192):
     check(lib().vil_attn_profile_begin(int(capacity)))
 

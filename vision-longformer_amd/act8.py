@@ -6,8 +6,6 @@ The reference's Mlp (src/models/msvit.py:17-34) keeps its input, fc1's output h 
 of 16 bits a token.  vil_mlp_act8 keeps the input and h in 8 bits (5 C of 1 1/32 bytes) and recomputes gelu from the packed h
 for fc2's weight gradient: 29 % of the bytes.  The forward result is the uncompressed one; gradients see the rounding.
 There is no eager fallback: CPU tensors or a missing library raise."""
-import ctypes
-
 import torch
 import torch.nn.functional as F
 
@@ -35,14 +33,6 @@ class Act8:
         return self.codes.numel() + self.scales.numel()
 
 
-def _p(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
-
-
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
 def _check(x, name):
     if x.dtype not in _DT:
         raise TypeError(f"{name} supports float32 / bfloat16 / float16; got {x.dtype}")
@@ -68,24 +58,24 @@ def _check_packed(p, name):
 def _rows(x):
     """x as (rows, cols) with contiguous columns and rows a fixed stride apart (a view where the layout allows it)"""
     cols = x.shape[-1]
-    x = x.reshape(x.numel() // cols if cols else 0, cols)
-    return x if (x.stride(1) == 1 or cols == 1) and (x.stride(0) >= cols or x.shape[0] <= 1) else x.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(x.numel() // cols if cols else 0, cols)
+    return x if x.is_contiguous() or ((x.stride(1) == 1 or cols == 1) and x.stride(0) >= cols) else x.contiguous()
 
 
 def _empty(x2):
     rows, cols = x2.shape
-    return (torch.empty(rows, cols, dtype=torch.int8, device=x2.device),
-            torch.empty(rows, -(-cols // BLOCK), dtype=torch.uint8, device=x2.device))
+    return x2.new_empty((rows, cols), dtype=torch.int8), x2.new_empty((rows, -(-cols // BLOCK)), dtype=torch.uint8)
 
 
 def vil_act8_pack(x):
     """x (..., C), fp32 / bf16 / fp16, in 8 bits: an Act8.  No gradient (the packed form is what a backward pass keeps)."""
     _check(x, "vil_act8_pack")
-    x2 = _rows(x.detach())
+    x2 = _rows(x)
+    rows, cols = x2.shape
     codes, scales = _empty(x2)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().vil_act8_pack(_p(x2), _DT[x.dtype], x2.shape[0], x2.shape[1], x2.stride(0), _p(codes), _p(scales),
-                                            _stream(x.device)))
+    _lib.launch(x.get_device(), _lib.lib().vil_act8_pack, x2.data_ptr(), _DT[x.dtype], rows, cols, x2.stride(0), codes.data_ptr(),
+                scales.data_ptr())
     return Act8(codes, scales, x.shape, x.dtype)
 
 
@@ -95,23 +85,23 @@ def vil_act8_unpack(packed, dtype=None):
     if dtype not in _DT:
         raise TypeError(f"vil_act8_unpack supports float32 / bfloat16 / float16; got {dtype}")
     _check_packed(packed, "vil_act8_unpack")
-    rows, cols = packed.codes.shape
-    y = torch.empty(packed.shape, dtype=dtype, device=packed.device)
-    with torch.cuda.device(packed.device):
-        _lib.check(_lib.lib().vil_act8_unpack(_p(packed.codes), _p(packed.scales), rows, cols, _p(y), _DT[dtype],
-                                              _stream(packed.device)))
+    codes = packed.codes
+    rows, cols = codes.shape
+    y = codes.new_empty(packed.shape, dtype=dtype)
+    _lib.launch(codes.get_device(), _lib.lib().vil_act8_unpack, codes.data_ptr(), packed.scales.data_ptr(), rows, cols, y.data_ptr(),
+                _DT[dtype])
     return y
 
 
 def vil_gelu_act8_fwd(h):
     """(gelu(h), h packed): the exact GELU and the packed pre-activation in one pass.  No gradient; see vil_gelu_act8."""
     _check(h, "vil_gelu_act8_fwd")
-    h2 = _rows(h.detach())
+    h2 = _rows(h)
+    rows, cols = h2.shape
     codes, scales = _empty(h2)
-    a = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    with torch.cuda.device(h.device):
-        _lib.check(_lib.lib().vil_gelu_act8_fwd(_p(h2), _DT[h.dtype], h2.shape[0], h2.shape[1], h2.stride(0), _p(a), _p(codes),
-                                                _p(scales), _stream(h.device)))
+    a = h2.new_empty(h.shape)
+    _lib.launch(h.get_device(), _lib.lib().vil_gelu_act8_fwd, h2.data_ptr(), _DT[h.dtype], rows, cols, h2.stride(0), a.data_ptr(),
+                codes.data_ptr(), scales.data_ptr())
     return a, Act8(codes, scales, h.shape, h.dtype)
 
 
@@ -123,12 +113,12 @@ def vil_gelu_act8_bwd(packed, da, want_act=True):
     _check_packed(packed, "vil_gelu_act8_bwd")
     if da.device != packed.device:
         raise RuntimeError(f"vil_gelu_act8_bwd: tensors on {da.device} and {packed.device}")
-    g2 = _rows(da.detach())
-    dh = torch.empty(da.shape, dtype=da.dtype, device=da.device)
-    a = torch.empty_like(dh) if want_act else None
-    with torch.cuda.device(da.device):
-        _lib.check(_lib.lib().vil_gelu_act8_bwd(_p(packed.codes), _p(packed.scales), _p(g2), _DT[da.dtype], g2.shape[0], g2.shape[1],
-                                                g2.stride(0), _p(dh), _p(a), _stream(da.device)))
+    g2 = _rows(da)
+    rows, cols = g2.shape
+    dh = g2.new_empty(da.shape)
+    a = g2.new_empty(da.shape) if want_act else None
+    _lib.launch(da.get_device(), _lib.lib().vil_gelu_act8_bwd, packed.codes.data_ptr(), packed.scales.data_ptr(), g2.data_ptr(),
+                _DT[da.dtype], rows, cols, g2.stride(0), dh.data_ptr(), a.data_ptr() if want_act else None)
     return dh, a
 
 

@@ -37,8 +37,8 @@ def grid_positions(*sides, nglo=0, device=None):
     return torch.cat([torch.zeros(int(nglo), len(sides), dtype=torch.int32), pos]).to(device)
 
 
-def _p(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _rows(t):
@@ -47,7 +47,7 @@ def _rows(t):
 
 
 def _check(q, k, wq, wk, positions, inv_freq, sections, layout, name):
-    """Everything a call can get wrong, before anything touches the device; returns (sections, layout code)."""
+    """Everything a call can get wrong, before anything touches the device."""
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError(f"{name}: q and k are (images, tokens, heads, channels)")
     B, N, _, M = q.shape
@@ -73,9 +73,7 @@ def _check(q, k, wq, wk, positions, inv_freq, sections, layout, name):
         raise ValueError(f"{name}: k_weight without k")
     if (positions is None) != (inv_freq is None) or (positions is None) != (sections is None):
         raise ValueError(f"{name}: positions, inv_freq and sections come together")
-    tensors = [q, k, wq, wk, positions, inv_freq]
     if positions is not None:
-        sections = tuple(int(n) for n in sections)
         if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) < 1 or 2 * sum(sections) > M:
             raise ValueError(f"{name}: sections {sections} of a head of {M} channels (1 to 4 axes, 1 to {M // 2} pairs in all)")
         if inv_freq.shape != (sum(sections),) or inv_freq.dtype not in _FREQ:
@@ -88,93 +86,144 @@ def _check(q, k, wq, wk, positions, inv_freq, sections, layout, name):
             raise ValueError(f"{name} has no gradient for positions and inv_freq")
     if layout not in _LAYOUTS:
         raise ValueError(f"{name}: layout {layout!r} (\"half\" or \"interleaved\")")
-    for t in tensors:
+    for t in (q, k, wq, wk, positions, inv_freq):
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{name} needs device tensors: the product path is the HIP kernels (libvilattn.so); there is no "
                                "CPU fallback")
         if t is not None and t.device != q.device:
             raise RuntimeError(f"{name}: tensors on {q.device} and {t.device}")
-    return sections
 
 
-def _desc(q, k, wq, wk, positions, inv_freq, cfg, yq=None, yk=None, gq=None, gk=None, dq=None, dk=None):
-    """cfg: (sections, layout, norm, eps)"""
-    sections, layout, norm, eps = cfg
-    B, N, Hq, M = q.shape
-    w = wq if wq is not None else wk
-    st = []
-    for t in (q, k, yq, yk, gq, gk, dq, dk):
-        st += t.stride()[:3] if t is not None else _NO_STRIDES
-    A, R, pos = 0, 0, (0, 0)
-    sec = (0, 0, 0, 0)
-    if positions is not None:
-        A, R = len(sections), sum(sections)
-        sec = sections + (0,) * (4 - A)
-        pos = (positions.stride(0) if positions.dim() == 3 else 0, positions.stride(-2))
-    return _lib.VilRopeDesc(B, N, Hq, k.shape[2] if k is not None else 0, M, R, A, sec, _LAYOUTS[layout], _DT[q.dtype],
-                            _POS[positions.dtype] if A else 0, _FREQ[inv_freq.dtype] if A else 0, int(norm),
-                            _DT[w.dtype] if w is not None else 0, eps, *st, *pos)
+def _dense(shape):
+    """strides (image, token, head) of a contiguous tensor"""
+    return (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
 
 
-def _launch(device, fn, desc, *tensors):
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        _lib.check(fn(ctypes.byref(desc), *[_p(t) for t in tensors], stream))
+class _Plan:
+    """What a call's layout decides (shapes, strides, types, options: nothing of any tensor's values or place): the checks have
+    passed, and the descriptors of the forward pass and of a backward pass with contiguous gradients are filled in.  A
+    training step makes the same few calls over and over; checking and filling take as long as the launch."""
+    __slots__ = ("base", "qs", "ks", "norm", "fwd", "bwd", "ws")
+
+    def __init__(self, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
+        B, N, Hq, M = self.qs = tuple(q.shape)
+        self.ks, self.norm = tuple(k.shape) if k is not None else None, norm
+        w = wq if wq is not None else wk
+        A, R, sec, self_pos = 0, 0, (0, 0, 0, 0), (0, 0)
+        if positions is not None:
+            A, R = len(sections), sum(sections)
+            sec = sections + (0,) * (4 - A)
+            self_pos = (positions.stride(0) if positions.dim() == 3 else 0, positions.stride(-2))
+        head = (B, N, Hq, k.shape[2] if k is not None else 0, M, R, A, sec, _LAYOUTS[layout], _DT[q.dtype],
+                _POS[positions.dtype] if A else 0, _FREQ[inv_freq.dtype] if A else 0, int(norm),
+                _DT[w.dtype] if w is not None else 0, eps)
+        x = q.stride()[:3] + (k.stride()[:3] if k is not None else _NO_STRIDES)
+        self.base = head, x, self_pos
+        dense = _dense(self.qs) + (_dense(self.ks) if k is not None else _NO_STRIDES)
+        self.fwd = _lib.VilRopeDesc(*head, *x, *dense, *_NO_STRIDES * 4, *self_pos)
+        self.bwd = self._bwd(dense, dense)
+        self.ws = _lib.lib().vil_qk_rope_workspace_bytes(ctypes.byref(self.fwd)) // 4
+
+    def _bwd(self, g, d):
+        head, x, pos = self.base
+        return _lib.VilRopeDesc(*head, *x, *_NO_STRIDES * 2, *g, *d, *pos)
+
+    def bwd_desc(self, gq, gk, dq=None, dk=None):
+        """of gradients (and outputs dq, dk; contiguous where they are None) with other strides"""
+        g = gq.stride()[:3] + (gk.stride()[:3] if gk is not None else _NO_STRIDES)
+        d = ((dq.stride()[:3] if dq is not None else _dense(self.qs)) +
+             ((dk.stride()[:3] if dk is not None else _dense(self.ks)) if self.ks else _NO_STRIDES))
+        return self._bwd(g, d)
 
 
-def _fwd(q, k, wq, wk, positions, inv_freq, cfg, yq, yk):
-    d = _desc(q, k, wq, wk, positions, inv_freq, cfg, yq=yq, yk=yk)
-    _launch(q.device, _lib.lib().vil_qk_rope_fwd, d, q, k, wq, wk, positions, inv_freq, yq, yk)
+_PLANS = {}
 
 
-def _bwd(q, k, wq, wk, positions, inv_freq, cfg, gq, gk, dq, dk, dwq, dwk):
-    d = _desc(q, k, wq, wk, positions, inv_freq, cfg, gq=gq, gk=gk, dq=dq, dk=dk)
-    L = _lib.lib()
-    ws = None
-    if dwq is not None or dwk is not None:
-        # (the call's own: two streams, or two captured graphs, never share it)
-        ws = torch.empty(L.vil_qk_rope_workspace_bytes(ctypes.byref(d)) // 4, dtype=torch.float32, device=q.device)
-    _launch(q.device, L.vil_qk_rope_bwd, d, gq, gk, q if cfg[2] else None, k if cfg[2] else None, wq, wk, positions, inv_freq,
-            dq, dk, dwq, dwk, ws)
+def _plan(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
+    index = q.get_device()
+    key = (q.shape, q.stride(), q.dtype, index, sections, layout, norm, eps,
+           (k.shape, k.stride(), k.dtype, k.get_device()) if k is not None else None,
+           (wq.shape, wq.dtype, wq.get_device()) if wq is not None else None,
+           (wk.shape, wk.dtype, wk.get_device()) if wk is not None else None,
+           (positions.shape, positions.stride(), positions.dtype, positions.get_device(), positions.requires_grad) if positions is not None else None,
+           (inv_freq.shape, inv_freq.dtype, inv_freq.get_device(), inv_freq.requires_grad) if inv_freq is not None else None)
+    plan = _PLANS.get(key)
+    if plan is None:
+        _check(q, k, wq, wk, positions, inv_freq, sections, layout, name)
+        plan = _Plan(q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps)
+        if len(_PLANS) >= 1024:                  # (a program with ever new shapes: start over)
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _fwd(plan, q, k, wq, wk, positions, inv_freq):
+    yq = q.new_empty(plan.qs)
+    yk = k.new_empty(plan.ks) if k is not None else None
+    _lib.launch(q.get_device(), _lib.lib().vil_qk_rope_fwd, plan.fwd, q.data_ptr(), _ptr(k), _ptr(wq), _ptr(wk), _ptr(positions),
+                _ptr(inv_freq), yq.data_ptr(), _ptr(yk))
+    return yq, yk
+
+
+def _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need_wq, need_wk):
+    """(dwq, dwk); dq and dk are written"""
+    dwq = wq.new_empty(wq.shape) if need_wq else None
+    dwk = wk.new_empty(wk.shape) if need_wk else None
+    # (the call's own workspace: two streams, or two captured graphs, never share it)
+    ws = gq.new_empty(plan.ws, dtype=torch.float32) if need_wq or need_wk else None
+    _lib.launch(gq.get_device(), _lib.lib().vil_qk_rope_bwd, desc, gq.data_ptr(), _ptr(gk), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
+                _ptr(positions), _ptr(inv_freq), dq.data_ptr(), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(ws))
+    return dwq, dwk
 
 
 class _QKRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, positions, inv_freq, cfg):
-        q, k = _rows(q), _rows(k) if k is not None else None
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
-        _fwd(q, k, wq, wk, positions, inv_freq, cfg, yq, yk)
-        # without the norm the gradient is the rotation back: the inputs are kept for their shapes only
-        ctx.save_for_backward(*((q, k) if cfg[2] else (None, None)), wq, wk, positions, inv_freq)
-        ctx.cfg, ctx.shapes = cfg, (q.shape, k.shape if k is not None else None)
-        return yq, yk
+    def forward(ctx, q, k, wq, wk, positions, inv_freq, plan):
+        ctx.plan = plan
+        # without the norm the gradient is the rotation back: the inputs need not be kept
+        ctx.save_for_backward(*((q, k) if plan.norm else (None, None)), wq, wk, positions, inv_freq)
+        return _fwd(plan, q, k, wq, wk, positions, inv_freq)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
-        qs, ks = ctx.shapes
-        gq, gk = _rows(gq), _rows(gk) if ks is not None else None
-        dq = torch.empty(qs, dtype=gq.dtype, device=gq.device)
-        dk = torch.empty(ks, dtype=gk.dtype, device=gk.device) if ks is not None else None
-        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
-        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
-        _bwd(q if q is not None else gq, k if k is not None else gk, wq, wk, positions, inv_freq, ctx.cfg, gq, gk, dq, dk, dwq, dwk)
+        plan, need = ctx.plan, ctx.needs_input_grad
+        desc = plan.bwd
+        if not gq.is_contiguous() or (gk is not None and not gk.is_contiguous()):
+            gq, gk = _rows(gq), _rows(gk) if gk is not None else None
+            desc = plan.bwd_desc(gq, gk)
+        dq = gq.new_empty(plan.qs)
+        dk = gk.new_empty(plan.ks) if gk is not None else None
+        dwq, dwk = _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need[2], need[3])
         return dq, dk, dwq, dwk, None, None, None
 
 
-def _positions(positions):
-    return positions if positions is None or positions.stride(-1) == 1 or positions.shape[-1] == 1 else positions.contiguous()
+def _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
+    """the call's plan and its tensors in the layouts that the kernels take"""
+    if q.dim() == 4:
+        q = _rows(q)
+    if k is not None and k.dim() == 4:
+        k = _rows(k)
+    if positions is not None:
+        if positions.dim() >= 2 and positions.stride(-1) != 1 and positions.shape[-1] != 1:
+            positions = positions.contiguous()
+        if inv_freq is not None and not inv_freq.is_contiguous():
+            inv_freq = inv_freq.contiguous()
+    if wq is not None and not wq.is_contiguous():
+        wq = wq.contiguous()
+    if wk is not None and not wk.is_contiguous():
+        wk = wk.contiguous()
+    sections = tuple(map(int, sections)) if sections is not None else None
+    return _plan(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps), q, k, wq, wk, positions, inv_freq
 
 
 def _apply(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
-    sections = _check(q, k, wq, wk, positions, inv_freq, sections, layout, name)
-    cfg = (sections, layout, norm, float(eps))
-    wq, wk = (w.contiguous() if w is not None else None for w in (wq, wk))
-    if inv_freq is not None:
-        inv_freq = inv_freq.contiguous()
-    yq, yk = _QKRope.apply(q, k, wq, wk, _positions(positions), inv_freq, cfg)
+    plan, *args = _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        yq, yk = _QKRope.apply(*args, plan)
+    else:
+        yq, yk = _fwd(plan, *args)
     return yq if k is None else (yq, yk)
 
 
@@ -198,4 +247,4 @@ def vil_qk_norm_rope(q, k=None, q_weight=None, k_weight=None, *, positions=None,
     fixed order.  Without positions (and inv_freq, sections): the norm alone.  Other arguments as vil_rope's."""
     if not eps >= 0:
         raise ValueError(f"vil_qk_norm_rope: eps {eps}")
-    return _apply("vil_qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, sections, layout, True, eps)
+    return _apply("vil_qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, sections, layout, True, float(eps))
