@@ -12,13 +12,18 @@ Differences by design (all numerically neutral):
     weights (longformer2d.py:127,211); here the first result is reused;
   * ``relative_position_index`` is still registered (state-dict compatibility)
     but the kernels compute the index arithmetically and never read it.
+
+Beyond the reference: ``qk_norm`` (a root-mean-square norm of every head of q and k) and ``rotary`` (q and k rotated by their
+row and column), off by default; layers with shared weights (``sharew``) and 1 to 4 global tokens.
 """
 import random
 
 import torch
 from torch import nn
 
-from .ops import vil_local_attention, vil_full_attention, vil_full_attention_qkv, vil_global_attention, FULL_MAX_G
+from .ops import (vil_local_attention, vil_full_attention, vil_full_attention_qkv, vil_global_attention, vil_rotary_attention_qkv,
+                  FULL_MAX_G)
+from .rotary import GridTurn, HeadNorm
 from .linear import VilLinear, vil_linear, vil_linear_pair
 
 
@@ -45,7 +50,7 @@ def build_relative_position_index(w):
 class Long2DSCSelfAttention(nn.Module):
     def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0., proj_drop=0., w=7, d=1,
                  autoregressive=False, sharew=False, nglo=1, only_glo=False, exact=0, autograd=False, rpe=False,
-                 mode=0):
+                 mode=0, qk_norm=False, rotary=False):
         super().__init__()
         assert d == 1, "Dilation is not supported!"
         assert not autoregressive, "Autoregressive is not supported yet!"
@@ -80,6 +85,11 @@ class Long2DSCSelfAttention(nn.Module):
                 self.proj_global = VilLinear(dim, dim)
         self.attn_drop = nn.Dropout(attn_drop)
         self.proj_drop = nn.Dropout(proj_drop)
+        self.q_norm = HeadNorm(self.head_dim) if qk_norm else None
+        self.k_norm = HeadNorm(self.head_dim) if qk_norm else None
+        self.turn = GridTurn(self.head_dim) if rotary else None
+        if (qk_norm or rotary) and not (self.fused_path_ok() if nglo >= 1 else False):
+            raise ValueError("qk_norm and rotary need the fused path: sharew=True, 1 to 4 global tokens, head_dim 8 / 16 / 32 / 48 / 64")
 
         if rpe:
             self.local_relative_position_bias_table = nn.Parameter(torch.zeros((4 * w - 1) ** 2, num_heads))
@@ -121,6 +131,8 @@ class Long2DSCSelfAttention(nn.Module):
             # the reference drops attention PROBABILITIES of local and global rows (longformer2d.py:186,224); the fused
             # kernels never materialise them.  No published config sets ATTN_DROP > 0: that case runs the reference's
             # own algorithm on the operator-level HIP kernels (scores materialised, as there)
+            if self.q_norm is not None or self.turn is not None:
+                raise RuntimeError("attn_drop > 0 with qk_norm or rotary: not supported in training")
             return self._forward_materialised(x, nx, ny)
         mode = self._resolve_mode()
         rs_dev = self.mode_dev is not None and self.mode > 0 and self.training
@@ -146,7 +158,13 @@ class Long2DSCSelfAttention(nn.Module):
                     wq, wkv = self.query.weight, self.kv.weight
                     bias = torch.cat([self.query.bias, self.kv.bias]) if self.query.bias is not None else None
                     qkv = vil_linear(x, torch.cat([wq, wkv], dim=0), bias)
-            if qkv is not None:
+            if self.q_norm is not None or self.turn is not None:
+                if qkv is None:
+                    qkv = torch.cat([self.query(x), self.kv(x)], dim=-1)
+                turn = self.turn.of(nx, ny, G, qkv.device) if self.turn is not None else {}
+                qw, kw_ = (self.q_norm.weight, self.k_norm.weight) if self.q_norm is not None else (None, None)
+                out = vil_rotary_attention_qkv(qkv, table, g2l, g2g, q_weight=qw, k_weight=kw_, norm=self.q_norm is not None, **turn, **kw)
+            elif qkv is not None:
                 out = vil_full_attention_qkv(qkv, table, g2l, g2g, **kw)
             else:
                 out = vil_full_attention(self.query(x), self.kv(x), table, g2l, g2g, **kw)

@@ -18,7 +18,9 @@ import torch.nn.functional as F
 from torch import nn
 
 from .longformer2d import Long2DSCSelfAttention, _trunc_normal_
-from .ops import vil_dense_attention, dense_family_supported, FULL_MAX_G
+from .ops import vil_dense_attention, vil_rotary_attention_qkv, dense_family_supported, FULL_MAX_G
+from .rotary import GridTurn, HeadNorm
+from .act8 import vil_mlp_act8
 from .layernorm import (VilLayerNorm, res_layernorm, res_layernorm_ok, tokens_layernorm, tokens_layernorm_ok,
                         pass_layernorm, pass_layernorm_ok)
 from .linear import VilLinear, vil_linear, vil_gelu_linear, vil_linear_gelu, expand_rows
@@ -133,8 +135,11 @@ class _TableGather(torch.autograd.Function):
 
 
 class Mlp(nn.Module):
-    def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0.):
+    """act8: keep the block's input and hidden pre-activation in 8 bits for the backward pass (act8.vil_mlp_act8: 29 % of the bytes)"""
+
+    def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0., act8=False):
         super().__init__()
+        self.act8 = act8
         self.fc1 = VilLinear(in_features, hidden_features or in_features)
         self.act = act_layer()
         self.fc2 = VilLinear(hidden_features or in_features, out_features or in_features)
@@ -142,6 +147,8 @@ class Mlp(nn.Module):
 
     def forward(self, x):
         if isinstance(self.act, nn.GELU) and self.act.approximate == "none" and (self.drop.p == 0.0 or not self.training):
+            if self.act8 and x.is_cuda and torch.is_grad_enabled():
+                return vil_mlp_act8(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias)
             # fc1 with the GELU in its epilogue where the weights-in-registers GEMM serves the shape (csrc/vil_gemm_skinny.hip),
             # fc2 with the GELU in front of it as one autograd node: its input gradient is ONE launch (dgrad GEMM with the
             # erf-GELU backward in the epilogue, csrc/vil_gemm_fused.hip)
@@ -155,9 +162,12 @@ class Attention(nn.Module):
     (nglo + wx*wy)-token sequence: the `s0` stages (reference msvit.py:37-120)."""
 
     def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0., proj_drop=0.,
-                 rpe=False, wx=14, wy=14, nglo=1):
+                 rpe=False, wx=14, wy=14, nglo=1, qk_norm=False, rotary=False):
         super().__init__()
         self.num_heads = num_heads
+        self.q_norm = HeadNorm(dim // num_heads) if qk_norm else None
+        self.k_norm = HeadNorm(dim // num_heads) if qk_norm else None
+        self.turn = GridTurn(dim // num_heads) if rotary else None
         self.scale = qk_scale or (dim // num_heads) ** -0.5
         self.qkv = VilLinear(dim, dim * 3, bias=qkv_bias)
         self.attn_drop = nn.Dropout(attn_drop)
@@ -203,8 +213,21 @@ class Attention(nn.Module):
         # used to fall to scaled_dot_product_attention with a materialised (H, N, N) bias)
         ok = (qkv.is_cuda and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32) and gx is not None and 0 <= nglo
               and nglo + gx * gy == N and (self.attn_drop.p == 0.0 or not self.training))
-        if ok and (dense_family_supported(qkv, gx, gy, nglo, H)
-                   or (gx == gy and gx <= 32 and nglo <= FULL_MAX_G and M in (16, 32, 48, 64))):
+        ok = ok and (dense_family_supported(qkv, gx, gy, nglo, H)
+                     or (gx == gy and gx <= 32 and nglo <= FULL_MAX_G and M in (16, 32, 48, 64)))
+        if self.q_norm is not None or self.turn is not None:
+            if not ok:
+                raise RuntimeError("qk_norm and rotary need device tensors and a grid that the attention kernels take")
+            turn = self.turn.of(gx, gy, nglo, qkv.device) if self.turn is not None else {}
+            qw, kw = (self.q_norm.weight, self.k_norm.weight) if self.q_norm is not None else (None, None)
+            rpe = self.rpe
+            out = vil_rotary_attention_qkv(qkv, self.local_relative_position_bias_table if rpe else None,
+                                           self.g2l_relative_position_bias if (rpe and nglo > 0) else None,
+                                           self.g2g_relative_position_bias if (rpe and nglo > 0) else None,
+                                           nx=gx, ny=gy, nglo=nglo, num_heads=H, scale=self.scale, q_weight=qw, k_weight=kw,
+                                           norm=self.q_norm is not None, **turn)
+            return self.proj_drop(self.proj(out))
+        if ok:
             # the dense attention of the s0 stages on its own HIP kernels (csrc/vil_attn_dense.hip:
             # head_dim 64, any grid) or, for the other head sizes, as the one-chunk case of the fused sliding-chunk kernels
             # -- bias table gathered in-kernel, no (H,N,N) bias tensor, no SDPA mask
@@ -323,17 +346,17 @@ class AttnBlock(nn.Module):
     def __init__(self, dim, num_heads, qkv_bias=False, qk_scale=None, drop=0., attn_drop=0., drop_path=0.,
                  norm_layer=nn.LayerNorm, attn_type='full', w=7, d=1, sharew=False, nglo=1, only_glo=False,
                  seq_len=None, num_feats=256, share_kv=False, sw_exact=0, rratio=2, rpe=False, wx=14, wy=14,
-                 mode=0):
+                 mode=0, qk_norm=False, rotary=False):
         super().__init__()
         self.norm = norm_layer(dim)
         if attn_type == 'full':
             self.attn = Attention(dim, num_heads=num_heads, qkv_bias=qkv_bias, qk_scale=qk_scale,
-                                  attn_drop=attn_drop, proj_drop=drop, rpe=rpe, wx=wx, wy=wy, nglo=nglo)
+                                  attn_drop=attn_drop, proj_drop=drop, rpe=rpe, wx=wx, wy=wy, nglo=nglo, qk_norm=qk_norm, rotary=rotary)
         elif attn_type in ('longformerhand', 'longformerauto'):
             self.attn = Long2DSCSelfAttention(
                 dim, exact=sw_exact, num_heads=num_heads, qkv_bias=qkv_bias, qk_scale=qk_scale,
                 attn_drop=attn_drop, proj_drop=drop, w=w, d=d, sharew=sharew, nglo=nglo, only_glo=only_glo,
-                autograd=(attn_type == 'longformerauto'), rpe=rpe, mode=mode)
+                autograd=(attn_type == 'longformerauto'), rpe=rpe, mode=mode, qk_norm=qk_norm, rotary=rotary)
         else:
             raise ValueError("Not supported attention type {}".format(attn_type))
         self.drop_path = DropPath(drop_path) if drop_path > 0. else nn.Identity()
@@ -346,11 +369,11 @@ class AttnBlock(nn.Module):
 
 class MlpBlock(nn.Module):
     def __init__(self, dim, out_dim=None, mlp_ratio=4., drop=0., drop_path=0., act_layer=nn.GELU,
-                 norm_layer=nn.LayerNorm):
+                 norm_layer=nn.LayerNorm, act8=False):
         super().__init__()
         self.drop_path = DropPath(drop_path) if drop_path > 0. else nn.Identity()
         self.norm = norm_layer(dim)
-        self.mlp = Mlp(dim, int(dim * mlp_ratio), out_dim, act_layer=act_layer, drop=drop)
+        self.mlp = Mlp(dim, int(dim * mlp_ratio), out_dim, act_layer=act_layer, drop=drop, act8=act8)
         self.shortcut = nn.Identity()
         if out_dim is not None and out_dim != dim:
             self.shortcut = nn.Sequential(VilLinear(dim, out_dim), nn.Dropout(drop))
@@ -375,10 +398,13 @@ def parse_arch(arch):
 
 
 class MsViT(nn.Module):
+    """qk_norm, rotary: every attention layer's q and k normalised per head / rotated by row and column (rotary.py); act8: the MLP
+    blocks keep their activations in 8 bits for the backward pass (act8.py).  All off by default."""
+
     def __init__(self, arch, img_size=512, in_chans=3, num_classes=1000, qkv_bias=True, qk_scale=None,
                  drop_rate=0., attn_drop_rate=0., drop_path_rate=0., norm_layer=partial(VilLayerNorm, eps=1e-6),
                  norm_embed=False, w=7, d=1, sharew=False, only_glo=False, share_kv=False,
-                 attn_type='longformerhand', sw_exact=0, mode=0, **args):
+                 attn_type='longformerhand', sw_exact=0, mode=0, qk_norm=False, rotary=False, act8=False, **args):
         super().__init__()
         self.num_classes = num_classes
         self.drop_path_rate = drop_path_rate
@@ -396,7 +422,7 @@ class MsViT(nn.Module):
 
         attn_args = dict(attn_type=attn_type, qkv_bias=qkv_bias, qk_scale=qk_scale, drop=drop_rate,
                          attn_drop=attn_drop_rate, w=w, d=d, sharew=sharew, only_glo=only_glo,
-                         share_kv=share_kv, sw_exact=sw_exact, norm_layer=norm_layer, mode=mode)
+                         share_kv=share_kv, sw_exact=sw_exact, norm_layer=norm_layer, mode=mode, qk_norm=qk_norm, rotary=rotary)
         dprs = torch.linspace(0, drop_path_rate, self.depth).split([c['n'] for c in self.layer_cfgs])
         side = img_size
         in_dim = in_chans
@@ -412,7 +438,7 @@ class MsViT(nn.Module):
                 blocks.append(AttnBlock(cfg['d'], cfg['h'], drop_path=float(dpr), seq_len=side * side + cfg['g'],
                                         rpe=not cfg['a'], wx=side, wy=side, **attn_args))
                 blocks.append(MlpBlock(cfg['d'], drop_path=float(dpr), mlp_ratio=4.0, norm_layer=norm_layer,
-                                       act_layer=nn.GELU, drop=drop_rate))
+                                       act_layer=nn.GELU, drop=drop_rate, act8=act8))
             setattr(self, "layer%d" % (i + 1), nn.Sequential(*blocks))
             in_dim = cfg['d']
         if self.num_layers == 3:

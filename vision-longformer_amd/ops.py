@@ -420,6 +420,40 @@ def vil_full_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, w, ng
     return _VilQKVAttention.apply(qkv, bias_table, g2l_bias, g2g_bias, cfg, backend or DEFAULT_BACKEND)
 
 
+def _dense_fwd(q, k, v, tab, g2l_f, g2g_f, cfg):
+    """(out, lse) of the dense kernel family; q / k / v are (B, N, C) views (last dim contiguous)"""
+    B, N, C = q.shape
+    out = torch.empty(B, N, C, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, cfg["H"], N + 1, dtype=torch.float32, device=q.device)     # [..., N]: max |v_k|^2 (see include/vil_attn.h)
+    d = _make_desc(q, k, v, out, cfg, "auto")
+    stream = ctypes.c_void_p(torch.cuda.current_stream(q.device).cuda_stream)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().vil_dense_attn_fwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(tab), _ptr(g2l_f),
+                                                 _ptr(g2g_f), _ptr(out), _ptr(lse), stream))
+    return out, lse
+
+
+def _dense_bwd(q, k, v, out, dout, lse, tab, g2l_f, g2g_f, dq, dk, dv, cfg):
+    """(dtab, dg2l, dg2g); dq / dk / dv are written"""
+    L = _lib.lib()
+    M = q.shape[-1] // cfg["H"]
+    dtab = torch.empty_like(tab) if tab is not None else None
+    dg2l = torch.empty_like(g2l_f) if g2l_f is not None else None
+    dg2g = torch.empty_like(g2g_f) if g2g_f is not None else None
+    d = _make_desc(q, k, v, out, cfg, "auto")
+    d.do_sb, d.do_st, d.do_sh = _strides(dout, M)
+    d.dq_sb, d.dq_st, d.dq_sh = _strides(dq, M)
+    d.dk_sb, d.dk_st, d.dk_sh = _strides(dk, M)
+    d.dv_sb, d.dv_st, d.dv_sh = _strides(dv, M)
+    ws = _workspace(d, 1, q.device, L.vil_dense_attn_workspace_bytes)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(q.device).cuda_stream)
+    with torch.cuda.device(q.device):
+        _lib.check(L.vil_dense_attn_bwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse),
+                                        _ptr(tab), _ptr(g2l_f), _ptr(g2g_f), _ptr(dq), _ptr(dk), _ptr(dv),
+                                        _ptr(dtab), _ptr(dg2l), _ptr(dg2g), _ptr(ws), stream))
+    return dtab, dg2l, dg2g
+
+
 class _VilDenseAttention(torch.autograd.Function):
     """The dense `Attention` of the s0 stages on its own kernel family (vil_dense_attn_fwd / _bwd, csrc/vil_attn_dense.hip):
     packed (B, N, 3C) projection in, (B, N, C) out, the gradient back as ONE (B, N, 3C) tensor; the global tokens are
@@ -431,16 +465,8 @@ class _VilDenseAttention(torch.autograd.Function):
         qkv = _last_contig(qkv)
         B, N, C3 = qkv.shape
         C = C3 // 3
-        H = cfg["H"]
-        q, k, v = qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:]
         tab, g2l_f, g2g_f = _f32c(table), _f32c(g2l), _f32c(g2g)
-        out = torch.empty(B, N, C, dtype=qkv.dtype, device=qkv.device)
-        lse = torch.empty(B, H, N + 1, dtype=torch.float32, device=qkv.device)     # [..., N]: max |v_k|^2 (see include/vil_attn.h)
-        d = _make_desc(q, k, v, out, cfg, "auto")
-        stream = ctypes.c_void_p(torch.cuda.current_stream(qkv.device).cuda_stream)
-        with torch.cuda.device(qkv.device):
-            _lib.check(_lib.lib().vil_dense_attn_fwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(tab), _ptr(g2l_f),
-                                                     _ptr(g2g_f), _ptr(out), _ptr(lse), stream))
+        out, lse = _dense_fwd(qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:], tab, g2l_f, g2g_f, cfg)
         ctx.save_for_backward(qkv, out, lse, tab, g2l_f, g2g_f)
         ctx.cfg = cfg
         ctx.dts = tuple(t.dtype if t is not None else None for t in (table, g2l, g2g))
@@ -450,28 +476,11 @@ class _VilDenseAttention(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, out, lse, tab, g2l_f, g2g_f = ctx.saved_tensors
         cfg = ctx.cfg
-        B, N, C3 = qkv.shape
-        C = C3 // 3
-        M = C // cfg["H"]
-        L = _lib.lib()
+        C = qkv.shape[-1] // 3
         dout = _last_contig(dout).to(qkv.dtype)
         dqkv = torch.empty_like(qkv)
-        q, k, v = qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:]
-        dq, dk, dv = dqkv[..., :C], dqkv[..., C:2 * C], dqkv[..., 2 * C:]
-        dtab = torch.empty_like(tab) if tab is not None else None
-        dg2l = torch.empty_like(g2l_f) if g2l_f is not None else None
-        dg2g = torch.empty_like(g2g_f) if g2g_f is not None else None
-        d = _make_desc(q, k, v, out, cfg, "auto")
-        d.do_sb, d.do_st, d.do_sh = _strides(dout, M)
-        d.dq_sb, d.dq_st, d.dq_sh = _strides(dq, M)
-        d.dk_sb, d.dk_st, d.dk_sh = _strides(dk, M)
-        d.dv_sb, d.dv_st, d.dv_sh = _strides(dv, M)
-        ws = _workspace(d, 1, qkv.device, L.vil_dense_attn_workspace_bytes)
-        stream = ctypes.c_void_p(torch.cuda.current_stream(qkv.device).cuda_stream)
-        with torch.cuda.device(qkv.device):
-            _lib.check(L.vil_dense_attn_bwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), _ptr(lse),
-                                            _ptr(tab), _ptr(g2l_f), _ptr(g2g_f), _ptr(dq), _ptr(dk), _ptr(dv),
-                                            _ptr(dtab), _ptr(dg2l), _ptr(dg2g), _ptr(ws), stream))
+        dtab, dg2l, dg2g = _dense_bwd(qkv[..., :C], qkv[..., C:2 * C], qkv[..., 2 * C:], out, dout, lse, tab, g2l_f, g2g_f,
+                                      dqkv[..., :C], dqkv[..., C:2 * C], dqkv[..., 2 * C:], cfg)
         tdt, ldt, gdt = ctx.dts
         return (dqkv, dtab.to(tdt) if dtab is not None else None, dg2l.to(ldt) if dg2l is not None else None,
                 dg2g.to(gdt) if dg2g is not None else None, None)
@@ -517,3 +526,101 @@ def vil_dense_attention(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, nglo, nu
         assert bias_table.shape[0] == side * side, "dense bias table must be ((2w-1)^2, H) with w = max(nx, ny)"
     cfg = _cfg(qkv.shape[-1] // 3, nx, ny, w, nglo, num_heads, -1, 0, scale, bias_side=side)
     return _VilQKVAttention.apply(qkv, bias_table, g2l_bias, g2g_bias, cfg, backend)
+
+
+class _VilRotaryAttention(torch.autograd.Function):
+    """vil_full_attention_qkv / vil_dense_attention with vil_rope or vil_qk_norm_rope on q and k in front, as one node on the
+    packed (B, N, 3C) projection: v is never copied, and the gradient comes back as one (B, N, 3C) tensor whose q and k parts
+    the rotation's backward pass writes straight from the attention's."""
+
+    @staticmethod
+    def forward(ctx, qkv, table, g2l, g2g, wq, wk, positions, inv_freq, cfg, turn, backend):
+        from . import rotary
+        B, N, C3 = qkv.shape
+        C, H = C3 // 3, cfg["H"]
+        q, k = _heads(qkv[..., :C], H), _heads(qkv[..., C:2 * C], H)
+        plan, q, k, wq, wk, positions, inv_freq = rotary._inputs("vil_rotary_attention_qkv", q, k, wq, wk, positions, inv_freq, *turn)
+        # the rotated q and k at the packed row's stride: the sliding-chunk kernels address k and v with one stride
+        qk = torch.empty(B, N, C3, dtype=qkv.dtype, device=qkv.device)
+        rotary._fwd(plan, q, k, wq, wk, positions, inv_freq, into=(_heads(qk[..., :C], H), _heads(qk[..., C:2 * C], H)))
+        tab, g2l_f, g2g_f = _f32c(table), _f32c(g2l), _f32c(g2g)
+        if backend == "dense":
+            (out, lse), lse_g = _dense_fwd(qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:], tab, g2l_f, g2g_f, cfg), None
+        else:
+            out, lse, lse_g = _full_fwd(qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:], tab, g2l_f, g2g_f, cfg, backend)
+        ctx.save_for_backward(qkv, qk, out, lse, lse_g, tab, g2l_f, g2g_f, wq, wk, positions, inv_freq)
+        ctx.cfg, ctx.plan, ctx.backend = cfg, plan, backend
+        ctx.dts = tuple(t.dtype if t is not None else None for t in (table, g2l, g2g))
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        from . import rotary
+        qkv, qk, out, lse, lse_g, tab, g2l_f, g2g_f, wq, wk, positions, inv_freq = ctx.saved_tensors
+        cfg, plan = ctx.cfg, ctx.plan
+        B, N, C3 = qkv.shape
+        C, H = C3 // 3, cfg["H"]
+        dout = _last_contig(dout).to(qkv.dtype)
+        dqkv = torch.empty_like(qkv)
+        gq, gk = (torch.empty(B, N, C, dtype=qkv.dtype, device=qkv.device) for _ in range(2))
+        views = (qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:])
+        if ctx.backend == "dense":
+            dtab, dg2l, dg2g = _dense_bwd(*views, out, dout, lse, tab, g2l_f, g2g_f, gq, gk, dqkv[..., 2 * C:], cfg)
+        else:
+            dtab, dg2l, dg2g = _full_bwd(*views, out, dout, lse, lse_g, tab, g2l_f, g2g_f, gq, gk, dqkv[..., 2 * C:], cfg, ctx.backend)
+        gq, gk, dq, dk = _heads(gq, H), _heads(gk, H), _heads(dqkv[..., :C], H), _heads(dqkv[..., C:2 * C], H)
+        need = ctx.needs_input_grad
+        dwq, dwk = rotary._bwd(plan, plan.bwd_desc(gq, gk, dq, dk), gq, gk, _heads(qkv[..., :C], H) if plan.norm else None,
+                               _heads(qkv[..., C:2 * C], H) if plan.norm else None, wq, wk, positions, inv_freq, dq, dk, need[4], need[5])
+        tdt, ldt, gdt = ctx.dts
+        return (dqkv, dtab.to(tdt) if dtab is not None else None, dg2l.to(ldt) if dg2l is not None else None,
+                dg2g.to(gdt) if dg2g is not None else None, dwq, dwk, None, None, None, None, None)
+
+
+def _heads(t, H):
+    return t.unflatten(-1, (H, t.shape[-1] // H))
+
+
+def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, nglo, num_heads, w=None, mode=0, exact=0, scale=None,
+                             backend=None, mode_dev=None, q_weight=None, k_weight=None, positions=None, inv_freq=None,
+                             sections=None, layout="half", norm=False, eps=1e-6):
+    """vil_full_attention_qkv (w = the window) or vil_dense_attention (w = None) of a packed (B, N, 3C) projection whose q and k
+    first pass vil_rope (norm=False) or vil_qk_norm_rope (norm=True; the weights may be None): one autograd node, v read in
+    place.  Arguments as those functions'; positions (N, axes) or (B, N, axes) cover the nglo global tokens, which come first."""
+    if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads):
+        raise ValueError(f"vil_rotary_attention_qkv: a packed projection of {num_heads} heads; got {tuple(qkv.shape)}")
+    if qkv.shape[1] != nglo + nx * ny:
+        raise ValueError(f"vil_rotary_attention_qkv: {qkv.shape[1]} tokens, {nglo} + {nx} x {ny} wanted")
+    if not norm and (q_weight is not None or k_weight is not None):
+        raise ValueError("vil_rotary_attention_qkv: weights without the norm")
+    if not norm and positions is None:
+        raise ValueError("vil_rotary_attention_qkv: neither a norm nor positions: vil_full_attention_qkv or vil_dense_attention")
+    _check_dev(qkv, "vil_rotary_attention_qkv")
+    qkv = _last_contig(qkv)
+    if not 0 <= nglo <= FULL_MAX_G or (w is not None and nglo == 0):
+        raise ValueError(f"vil_rotary_attention_qkv: nglo {nglo}")
+    if nglo == 0:
+        g2l_bias = g2g_bias = None
+    C = qkv.shape[-1] // 3
+    backend = backend or DEFAULT_BACKEND
+    if w is not None:
+        if exact not in (0, 1, -1) or (exact == 1 and mode != 0):
+            raise ValueError("longsc exact should be in [0,1,-1]!")
+        cfg = _cfg(C, nx, ny, w, nglo, num_heads, mode, exact, scale)
+        if mode_dev is not None:
+            assert mode > 0 and mode_dev.dtype == torch.int32 and mode_dev.is_cuda
+            cfg["mode_dev"] = mode_dev.data_ptr()
+    else:
+        dense = (backend in ("auto", "dense") and dense_family_supported(qkv, nx, ny, nglo, num_heads)
+                 and (bias_table is None or bias_table.shape[0] == (2 * int(nx) - 1) * (2 * int(ny) - 1)))
+        if backend == "dense" and not dense:
+            raise RuntimeError("vil_rotary_attention_qkv: the dense kernel family does not take this problem")
+        side = 2 * max(int(nx), int(ny)) - 1
+        if not dense and bias_table is not None and bias_table.shape[0] != side * side:
+            raise ValueError(f"vil_rotary_attention_qkv: a bias table of {side} x {side} rows wanted")
+        backend = "dense" if dense else backend
+        cfg = _cfg(C, nx, ny, max(int(nx), int(ny)), nglo, num_heads, -1, 0, scale,
+                   bias_side=side if bias_table is not None and not dense else 0)
+    sections = tuple(int(n) for n in sections) if sections is not None else None
+    return _VilRotaryAttention.apply(qkv, bias_table, g2l_bias, g2g_bias, q_weight, k_weight, positions, inv_freq, cfg,
+                                     (sections, layout, bool(norm), float(eps)), backend)

@@ -128,6 +128,12 @@ class _Plan:
         head, x, pos = self.base
         return _lib.VilRopeDesc(*head, *x, *_NO_STRIDES * 2, *g, *d, *pos)
 
+    def fwd_desc(self, yq, yk):
+        """of outputs with other strides"""
+        head, x, pos = self.base
+        y = yq.stride()[:3] + (yk.stride()[:3] if yk is not None else _NO_STRIDES)
+        return _lib.VilRopeDesc(*head, *x, *y, *_NO_STRIDES * 4, *pos)
+
     def bwd_desc(self, gq, gk, dq=None, dk=None):
         """of gradients (and outputs dq, dk; contiguous where they are None) with other strides"""
         g = gq.stride()[:3] + (gk.stride()[:3] if gk is not None else _NO_STRIDES)
@@ -157,10 +163,16 @@ def _plan(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
     return plan
 
 
-def _fwd(plan, q, k, wq, wk, positions, inv_freq):
-    yq = q.new_empty(plan.qs)
-    yk = k.new_empty(plan.ks) if k is not None else None
-    _lib.launch(q.get_device(), _lib.lib().vil_qk_rope_fwd, plan.fwd, q.data_ptr(), _ptr(k), _ptr(wq), _ptr(wk), _ptr(positions),
+def _fwd(plan, q, k, wq, wk, positions, inv_freq, into=None):
+    """(yq, yk), contiguous, or `into` two tensors with other strides"""
+    if into is None:
+        yq = q.new_empty(plan.qs)
+        yk = k.new_empty(plan.ks) if k is not None else None
+        desc = plan.fwd
+    else:
+        yq, yk = into
+        desc = plan.fwd_desc(yq, yk)
+    _lib.launch(q.get_device(), _lib.lib().vil_qk_rope_fwd, desc, q.data_ptr(), _ptr(k), _ptr(wq), _ptr(wk), _ptr(positions),
                 _ptr(inv_freq), yq.data_ptr(), _ptr(yk))
     return yq, yk
 
@@ -185,8 +197,11 @@ class _QKRope(torch.autograd.Function):
         return _fwd(plan, q, k, wq, wk, positions, inv_freq)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
+        return _QKRope.second(ctx, gq, gk) if torch.is_grad_enabled() else _QKRope.first(ctx, gq, gk)
+
+    @staticmethod
+    def first(ctx, gq, gk):
         q, k, wq, wk, positions, inv_freq = ctx.saved_tensors
         plan, need = ctx.plan, ctx.needs_input_grad
         desc = plan.bwd
@@ -197,6 +212,9 @@ class _QKRope(torch.autograd.Function):
         dk = gk.new_empty(plan.ks) if gk is not None else None
         dwq, dwk = _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need[2], need[3])
         return dq, dk, dwq, dwk, None, None, None
+
+    # under create_graph: the same values, and an error where a second derivative is asked of them
+    second = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, gq, gk: _QKRope.first(ctx, gq, gk)))
 
 
 def _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
@@ -248,3 +266,36 @@ def vil_qk_norm_rope(q, k=None, q_weight=None, k_weight=None, *, positions=None,
     if not eps >= 0:
         raise ValueError(f"vil_qk_norm_rope: eps {eps}")
     return _apply("vil_qk_norm_rope", q, k, q_weight, k_weight, positions, inv_freq, sections, layout, True, float(eps))
+
+
+class HeadNorm(torch.nn.Module):
+    """The (M,) weight of a root-mean-square norm that every head of q, or of k, shares (a parameter `weight`, which
+    MsViT.no_weight_decay's rule leaves undecayed); the norm itself runs in the attention's node."""
+
+    def __init__(self, head_dim):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.ones(head_dim))
+
+
+class GridTurn:
+    """The rotation of a layer on an nx x ny token grid behind nglo global tokens: half of a head's pairs turn with the row,
+    half with the column (the rows take the odd one).  `of(nx, ny, nglo, device)` gives vil_rotary_attention_qkv's positions,
+    inv_freq, sections and layout; each grid's tensors are made once (before a stream capture: the layer's first run)."""
+
+    def __init__(self, head_dim, base=10000.0, layout="half"):
+        if head_dim % 4:
+            raise ValueError(f"GridTurn: a head of {head_dim} channels (a multiple of 4: two axes)")
+        if layout not in _LAYOUTS:
+            raise ValueError(f"GridTurn: layout {layout!r}")
+        pairs = head_dim // 2
+        self.sections, self.base, self.layout = (pairs - pairs // 2, pairs // 2), base, layout
+        self._made = {}
+
+    def of(self, nx, ny, nglo, device):
+        key = (int(nx), int(ny), int(nglo), device)
+        made = self._made.get(key)
+        if made is None:
+            with torch.inference_mode(False):            # (an evaluation may come first, and training save them)
+                made = self._made[key] = dict(positions=grid_positions(nx, ny, nglo=nglo, device=device), sections=self.sections,
+                                              inv_freq=rotary_frequencies(self.sections, self.base, device), layout=self.layout)
+        return made
