@@ -304,3 +304,48 @@ def test_row_stride_past_32_bits_of_offset():
     buf[:, 8:104] = x
     p, q = act8.vil_act8_pack(buf[:, 8:104]), act8.vil_act8_pack(x)
     assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (2, 0, 64)])
+def test_mlp_of_an_empty_batch(shape):
+    _, w1, b1, w2, b2 = mlp_args(4, 64, 256, torch.bfloat16)
+    x = torch.zeros(*shape, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = act8.vil_mlp_act8(x, w1, b1, w2, b2)
+    assert y.shape == (*shape[:-1], 64)
+    for g, v in zip(torch.autograd.grad(y, (x, w1, b1, w2, b2), torch.ones_like(y)), (x, w1, b1, w2, b2)):
+        assert g.shape == v.shape and bool((g == 0).all())
+
+
+def test_mlp_of_a_vector_and_of_a_broadcast_gradient():
+    x, w1, b1, w2, b2 = mlp_args(40, 64, 256, torch.bfloat16)
+    y = act8.vil_mlp_act8(x, w1, b1, w2, b2)
+    one = torch.autograd.grad(y, (x, w1, b1, w2, b2), torch.ones_like(y))
+    y = act8.vil_mlp_act8(x, w1, b1, w2, b2)
+    for a, b in zip(one, torch.autograd.grad(y, (x, w1, b1, w2, b2), torch.ones((), device="cuda", dtype=y.dtype).expand_as(y))):
+        # (a broadcast gradient takes the products of another kernel: 12 half steps of the rms, as above)
+        assert float((a - b).float().norm()) <= 12 * 2.0 ** -8 * float(a.float().norm())
+    v = x[0, 0].detach().requires_grad_()
+    y = act8.vil_mlp_act8(v, w1, b1, w2, b2)
+    assert y.shape == (64,) and torch.autograd.grad(y, v, torch.ones_like(y))[0].shape == v.shape
+
+
+def test_non_finite_gradients_stay_visible():
+    """fp16 training: an infinite or NaN incoming gradient, or an overflowed pre-activation, is not finite afterwards either"""
+    h = data(4, 64, torch.float16)
+    da = torch.ones_like(h)
+    da[1, 3], da[2, 5] = float("inf"), float("nan")
+    h[3, 7] = float("inf")
+    _, h8 = act8.vil_gelu_act8_fwd(h)
+    dh, again = act8.vil_gelu_act8_bwd(h8, da)
+    bad = ~torch.isfinite(dh)
+    assert bool(bad[1, 3]) and bool(bad[2, 5]) and bool(bad[3, :32].all()) and int(bad.sum()) == 34 and bool(again[3, :32].isnan().all())
+
+
+def test_rows_behind_and_channels_beside_are_left_alone():
+    buf = torch.zeros(6, 200, device="cuda", dtype=torch.bfloat16)
+    buf[:4, 16:113] = data(4, 97, torch.bfloat16)
+    keep = buf.clone()
+    x = buf[:4, 16:113]
+    a, h8 = act8.vil_gelu_act8_fwd(x)
+    p = act8.vil_act8_pack(x)
+    assert torch.equal(buf, keep) and torch.equal(p.codes, act8.vil_act8_pack(x.contiguous()).codes) and torch.equal(h8.codes, p.codes)

@@ -364,3 +364,119 @@ def test_long_token_axis_past_32_bits_of_offset():
 def test_the_c_entry_reports_the_launch_contract():
     d = _lib.VilRopeDesc()
     assert _lib.lib().vil_qk_rope_fwd(ctypes.byref(d), *([None] * 9)) < 0
+
+
+def both_ways(q, k, wq, wk, gq, gk, **kw):
+    leaves = [v.detach().requires_grad_() for v in (q, k, wq, wk)]
+    y = rotary.vil_qk_norm_rope(*leaves, eps=1e-5, **kw)
+    return [v.detach() for v in y], torch.autograd.grad(y, leaves, (gq, gk))
+
+
+def against_formulas(q, k, wq, wk, gq, gk, pos, f, sections, layout="half"):
+    (yq, yk), (dq, dk, dwq, dwk) = both_ways(q, k, wq, wk, gq, gk, positions=pos, inv_freq=f, sections=sections, layout=layout)
+    cos, sin = angles(pos, f, sections)
+    for x, w, g, y, d, dw in ((q, wq, gq, yq, dq, dwq), (k, wk, gk, yk, dk, dwk)):
+        ref = reference(x.detach().double(), w.double(), g.double(), cos, sin, layout, True, 1e-5)
+        check("y", y, *ref["y"], x.dtype)
+        check("dx", d, *ref["dx"], x.dtype)
+        check("dw", dw, *ref["dw"], w.dtype)
+
+
+@pytest.mark.parametrize("B,N", [(1500, 3), (70000, 1), (3, 700)])
+@pytest.mark.parametrize("kind", ["grid", "stream"])
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_many_images_and_many_tiles(B, N, kind, layout):
+    """more images than the grid's second axis or the backward's workgroups hold, in a layout whose images are one run of tokens and
+    in one where they are not; positions shared and each image's own"""
+    H, M, t = 2, 16, torch.bfloat16
+    q, k, gq, gk, wq, wk = make(B, N, H, H, M, t, False)
+    if layout == "heads":
+        q, k, gq, gk = (v.transpose(1, 2).contiguous().transpose(1, 2) for v in (q, k, gq, gk))
+    pos = positions_of("grid" if kind == "grid" else "far", B, N, 2)
+    against_formulas(q, k, wq, wk, gq, gk, pos, rotary.rotary_frequencies((4, 4), device="cuda"), (4, 4))
+
+
+@pytest.mark.parametrize("how", ["8_byte_offset", "heads_shared_by_stride_0", "16_mb_rows", "one_position_for_all"])
+def test_more_layouts(how):
+    B, N, H, M, t = 2, 9, 4, 64, torch.float16
+    q, k, gq, gk, wq, wk = make(B, N, H, H, M, t, False)
+    pos = positions_of("scaled", B, N, 2)
+    if how == "8_byte_offset":
+        flat = torch.zeros(2, B * N * H * M + 4, device="cuda", dtype=t)
+        flat[:, 4:] = torch.stack([q, k]).view(2, -1)
+        q, k = flat[0, 4:].view(B, N, H, M), flat[1, 4:].view(B, N, H, M)
+    elif how == "heads_shared_by_stride_0":
+        q, k = q[:, :, :1].expand(B, N, H, M), k[:, :, :1].expand(B, N, H, M)
+    elif how == "16_mb_rows":
+        buf = torch.zeros(N, 2 ** 23, device="cuda", dtype=t)
+        B, q, k, gq, gk, pos = 1, q[:1], k[:1], gq[:1], gk[:1], pos[:1]
+        buf[:, :2 * H * M] = torch.cat([q, k], 2).view(N, -1)
+        q, k = buf[:, :H * M].view(1, N, H, M), buf[:, H * M:2 * H * M].view(1, N, H, M)
+    else:
+        pos = pos[:1, :1].expand(B, N, 2)
+    against_formulas(q, k, wq, wk, gq, gk, pos, rotary.rotary_frequencies((16, 16), device="cuda"), (16, 16))
+
+
+def test_gradient_of_a_broadcast_input():
+    """one head of k serving four by expand(): its gradient is the sum of theirs, each rounded once: 4 half steps and the sum's"""
+    q, k, gq, gk, wq, wk = make(2, 9, 4, 4, 32, torch.bfloat16, False)
+    pos, f = positions_of("grid", 2, 9, 2), rotary.rotary_frequencies((8, 8), device="cuda")
+    kw = dict(positions=pos, inv_freq=f, sections=(8, 8))
+    one = k[:, :, :1].detach().requires_grad_()
+    y = rotary.vil_qk_norm_rope(one.expand(2, 9, 4, 32), None, wk, **kw)
+    got, = torch.autograd.grad(y, one, gk)
+    four = k[:, :, :1].expand(2, 9, 4, 32).detach().requires_grad_()
+    parts, = torch.autograd.grad(rotary.vil_qk_norm_rope(four, None, wk, **kw), four, gk)
+    ref = parts.double().sum(2, keepdim=True)
+    assert bool(((got.double() - ref).abs() <= 2.0 ** -8 * parts.double().abs().sum(2, keepdim=True) + 1e-30).all())
+
+
+def test_second_derivatives_are_refused_and_create_graph_is_not():
+    q, k, gq, gk, wq, wk = make(1, 5, 2, 2, 32, torch.float32, False)
+    pos, f = positions_of("grid", 1, 5, 2), rotary.rotary_frequencies((8, 8), device="cuda")
+    q = q.requires_grad_()
+    y = rotary.vil_qk_norm_rope(q, None, wq, positions=pos, inv_freq=f, sections=(8, 8))
+    first, = torch.autograd.grad(y, q, gq, retain_graph=True)
+    again, = torch.autograd.grad(y, q, gq, create_graph=True)
+    assert torch.equal(first, again)
+    with pytest.raises(RuntimeError):
+        again.sum().backward()
+
+
+def test_two_streams_at_once():
+    """calls on two streams in flight together, each with its own weights' gradients: nothing is shared between them"""
+    pos, f = positions_of("grid", 16, 785, 2), rotary.rotary_frequencies((16, 16), device="cuda")
+    kw = dict(positions=pos, inv_freq=f, sections=(16, 16))
+    sets = [make(16, 785, 3, 3, 64, torch.bfloat16, True, seed) for seed in (0, 1)]
+
+    def step(v):
+        y, g = both_ways(v[0], v[1], v[4], v[5], v[2], v[3], **kw)
+        return [*y, *g]
+
+    want = [step(v) for v in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(sets[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for turn in got[i]:
+            for a, b in zip(turn, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_same_tensor_twice_and_rows_behind_the_last():
+    """q and k one tensor: both gradients arrive; a slice's neighbours in memory are left as they were"""
+    buf = torch.randn(2, 12, 3, 32, device="cuda")
+    keep = buf.clone()
+    x = buf[:, :9].detach().requires_grad_()
+    pos, f = positions_of("grid", 2, 9, 2), rotary.rotary_frequencies((8, 8), device="cuda")
+    kw = dict(positions=pos, inv_freq=f, sections=(8, 8))
+    a, b = rotary.vil_rope(x, x, **kw)
+    assert torch.equal(a, b)
+    one, = torch.autograd.grad(a, x, torch.ones_like(a), retain_graph=True)
+    two, = torch.autograd.grad((a, b), x, (torch.ones_like(a), torch.ones_like(b)))
+    assert torch.equal(two, 2 * one) and torch.equal(buf, keep)
