@@ -162,9 +162,9 @@ class _MlpAct8Fn(torch.autograd.Function):
         x2 = _rows(x)
         a, h8 = vil_gelu_act8_fwd(_linear(x2, w1, b1))
         y = _linear(a, w2, b2)
-        x8 = vil_act8_pack(x2)
-        ctx.save_for_backward(x8.codes, x8.scales, h8.codes, h8.scales, w1, w2)
-        ctx.was = (x.shape, x8.shape, h8.shape, x.dtype, h8.dtype, b1 is not None, b2 is not None)
+        x8 = vil_act8_pack(x2) if ctx.needs_input_grad[1] else None      # (x serves fc1's weight gradient alone)
+        ctx.save_for_backward(*((x8.codes, x8.scales) if x8 is not None else (None, None)), h8.codes, h8.scales, w1, w2)
+        ctx.was = (x.shape, x2.shape, h8.shape, x.dtype, h8.dtype, b1 is not None, b2 is not None)
         return y.view(*x.shape[:-1], w2.shape[0])
 
     @staticmethod

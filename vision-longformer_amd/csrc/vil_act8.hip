@@ -14,6 +14,10 @@
 // in t = 1 / (1 + p z), fitted to the least maximum of the RELATIVE error over z in [0, 10]: the negative tail keeps its
 // digits, which 1 - erf would cancel.  Six terms: 5.2e-6, against a half step of 2^-11 (fp16) and 2^-9 (bf16); eight terms for
 // fp32: 9e-8, 4e-7 with the rounding of the evaluation.
+//
+// Bound: memory, the GELU nearly as much by vector instructions.  bf16, 401536 x 384, MI355X: GELU forward 134 us (775 MB, 5.8 TB/s;
+// 103 us of it issue vector instructions), backward 189 us (1.08 GB, 5.7 TB/s; 121); pack + unpack of 100480 x 192 21 us (5.4 TB/s, partly
+// from the last-level cache).  A large copy runs at 5.3 TB/s.
 #include "vil_internal.h"
 
 namespace {

@@ -10,6 +10,11 @@
 // Angles.  pos * freq / 2 pi is taken in fp64 and reduced to a quarter turn there, so that positions far into a stream keep
 // their angle (fp32 would lose 2^-24 of 10^5 radians: the whole fractional turn); sine and cosine of the remainder in
 // [-pi/4, pi/4] are their Taylor series in fp32 (next terms 2e-9 and 1e-10).
+//
+// Bound: memory.  Forward 2, backward 3 bytes a byte of q and k.  bf16, 128 x 3137 tokens, 3 heads of 32 of a packed projection (154 MB of
+// q and k), MI355X: norm forward 68 us = 4.5 TB/s (192-byte slices at a stride of 576 share their end lines with v: 1.18 times
+// the bytes are read), norm backward 87 us = 5.3 TB/s, dw 4 us; rotation alone at 32 x 9217: 50 us = 4.6 TB/s each way; a large
+// copy runs at 5.3.
 #include "vil_internal.h"
 #include <string.h>
 
@@ -296,7 +301,8 @@ template <typename T, int CH> __device__ __forceinline__ void ro_store(char* bas
 }
 
 // Head rows of a tile, one side: IPT rows to a thread and step, the next step's loads issued before this one's arithmetic, so that
-// loads stay under way while a wave computes (without it the forward pass took 82 us where a copy of the same slices takes 61).
+// loads stay under way while a wave computes (norm forward at 128 x 3137 x 3 heads of 32: 82 us without, 73 with it; a copy of the
+// same slices takes 61).
 // Rows past the end load the last row again and store nothing.
 template <typename T, int CH, int LPR, int IPT> struct RoRows {
   static constexpr int ROWS = RO_THREADS / LPR;
@@ -534,7 +540,7 @@ int ro_chunk(const RoParams& p, int dtype, bool bwd_norm) {
         small = small && st >= 0 && st * size < (1 << 24);
       }
       // (offsets in a tile stay under 2^32: the heads under 2^30 here, the tokens in ro_plan)
-      small = small && S.H * S.x_sh * size < (1 << 30) && S.H * S.y_sh * size < (1 << 30) && (!bwd_norm || S.H * S.g_sh * size < (1 << 30));
+      small = small && S.H <= (1 << 15) && S.H * S.x_sh * size < (1 << 30) && S.H * S.y_sh * size < (1 << 30) && (!bwd_norm || S.H * S.g_sh * size < (1 << 30));
       bits |= (uintptr_t)S.x | (uintptr_t)S.y | (uintptr_t)((S.x_sb | S.y_sb) * size);
       if (bwd_norm) bits |= (uintptr_t)S.g | (uintptr_t)(S.g_sb * size);
     }
@@ -580,9 +586,9 @@ void ro_plan(RoParams& p, int size, int wave_rows, int step, int64_t want, int r
     const int64_t units = (int64_t)p.ntiles * p.nseg, most = want * rounds, spg = (units + most - 1) / most;
     p.spg = spg > p.nseg ? p.nseg : (int)spg;
   }
-  for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic(p.s[i].H);      // rows of a tile <= 2^16, heads < 2^7
-  p.n_magic = p.flat && p.N < p.tile ? ro_magic(p.N) : 0;                   // both <= 2^9
-  p.r_magic = p.R ? ro_magic(p.R) : 0;                                      // angles <= 2^11 or pairs of one token
+  for (int i = 0; i < p.sides; ++i) p.h_magic[i] = ro_magic(p.s[i].H);      // x: rows of a tile, <= 2^11 or the heads of one token
+  p.n_magic = p.flat && p.N < p.tile ? ro_magic(p.N) : 0;                   // x < 2^10, N < 2^9
+  p.r_magic = p.R ? ro_magic(p.R) : 0;                                      // x: angles of a tile, <= 2^11
 }
 
 template <typename T, int CH, int LPR, bool NORM>
