@@ -491,6 +491,14 @@ int vil_act8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t x_ro
 int vil_act8_unpack(const void* codes, const void* scales, int64_t rows, int cols, void* y, int dtype, void* stream);
 int vil_gelu_act8_fwd(const void* h, int dtype, int64_t rows, int cols, int64_t h_row_stride, void* a, void* codes, void* scales,
                       void* stream);
+/* The same around the MLP block's products (bf16, row strides in elements; contracts of vil_gemm_gelu_bf16 and
+ * vil_gemm_dgelu_bf16; codes 8-byte, for _dgelu scales 2-byte aligned):
+ *   _gelu_act8:  h = x . w^T + bias rounded to bf16 and never stored: a = gelu(h) and h packed
+ *   _dgelu_act8: with v = the values of the packed h, dh = (dy . w) * gelu'(v) and a = gelu(v), both with out_row_stride */
+int vil_gemm_gelu_act8_bf16(const void* x, const void* w, const void* bias, void* a, void* codes, void* scales, int64_t T, int K, int N,
+                            int64_t x_row_stride, int64_t a_row_stride, void* stream);
+int vil_gemm_dgelu_act8_bf16(const void* dy, const void* w, const void* codes, const void* scales, void* dh, void* a, int64_t T, int K,
+                             int N, int64_t dy_row_stride, int64_t out_row_stride, void* stream);
 int vil_gelu_act8_bwd(const void* codes, const void* scales, const void* da, int dtype, int64_t rows, int cols,
                       int64_t da_row_stride, void* dh, void* a, void* stream);
 

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from vision_longformer_amd import act8
+from vision_longformer_amd import _lib, act8
 
 pytestmark = pytest.mark.gpu
 TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -349,3 +349,134 @@ def test_rows_behind_and_channels_beside_are_left_alone():
     a, h8 = act8.vil_gelu_act8_fwd(x)
     p = act8.vil_act8_pack(x)
     assert torch.equal(buf, keep) and torch.equal(p.codes, act8.vil_act8_pack(x.contiguous()).codes) and torch.equal(h8.codes, p.codes)
+
+
+@pytest.mark.parametrize("T", [1, 127, 1100, 2177])
+@pytest.mark.parametrize("K,N", [(384, 1536), (96, 384), (192, 768), (416, 128)])
+@pytest.mark.parametrize("entry", ["fwd", "bwd"])
+def test_products_with_the_packed_form_in_their_epilogue(entry, K, N, T):
+    """fc1 with GELU and packing, fc2's input gradient with the GELU's backward.  The operands are small multiples of a power of two,
+    so that a sum of the products is exact in 32 bits (below 2^24 units) in any order: codes and scales are those of the product
+    rounded to bf16, a and dh are off by the GELU's tolerances alone.  One row has a NaN, one an infinity."""
+    L, t = _lib.lib(), torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(T + K)
+    whole = lambda m, *size: torch.randint(-m, m + 1, size, generator=gen, device="cuda").float()
+    x, w, b = whole(8, T, K).to(t), (whole(8, N, K) / 512).to(t), (whole(200, N) / 512).to(t)
+    if T > 100:
+        x[3, 5], x[T - 1, 7] = float("nan"), float("inf")
+    codes = torch.full((T + 1, N), 77, device="cuda", dtype=torch.int8)
+    scales = torch.full((T + 1, N // 32), 77, device="cuda", dtype=torch.uint8)
+    a = torch.full((T + 1, N + 8), 7.0, device="cuda", dtype=t)                        # a row stride of its own, a row behind the last
+    if entry == "fwd":
+        _lib.launch(0, L.vil_gemm_gelu_act8_bf16, x.data_ptr(), w.data_ptr(), b.data_ptr(), a.data_ptr(), codes.data_ptr(), scales.data_ptr(), T, K, N, K, N + 8)
+        h = (x.cpu().double() @ w.cpu().double().t() + b.cpu().double()).to(t)
+        want = act8.vil_act8_pack(h.cuda())
+        assert torch.equal(scales[:T], want.scales) and torch.equal(codes[:T], want.codes)
+        assert bool((scales[T] == 77).all()) and bool((codes[T] == 77).all())
+        hd = h.cuda().double()
+        fine = torch.isfinite(hd).all(1)
+        assert int(fine.sum()) >= T - 2
+        hf = hd[fine]
+        check("a", a[:T, :N][fine], gelu64(hf)[0], hf.abs() * gelu_tolerance(hf, t)[0], t)
+    else:
+        w = w.t().contiguous()
+        h8 = act8.vil_act8_pack(2 * data(T, N, t, 4))
+        dh = torch.full((T + 1, N + 8), 7.0, device="cuda", dtype=t)
+        _lib.launch(0, L.vil_gemm_dgelu_act8_bf16, x.data_ptr(), w.data_ptr(), h8.codes.data_ptr(), h8.scales.data_ptr(), dh.data_ptr(),
+                    a.data_ptr(), T, K, N, K, N + 8)
+        v = act8.vil_act8_unpack(h8, torch.float32).double()
+        act, slope, _, _, pdf = gelu64(v)
+        g = (x.cpu().double() @ w.cpu().double()).cuda()
+        fine = torch.isfinite(g).all(1)
+        assert int(fine.sum()) >= T - 2
+        c, d = gelu_tolerance(v, t)
+        check("a", a[:T, :N], act, v.abs() * c, t)
+        check("dh", dh[:T, :N][fine], (g * slope)[fine], (g.abs() * (c + v.abs() * d + 2.0 ** -22 * (slope.abs() + v.abs() * pdf)))[fine], t)
+        if T > 100:
+            assert bool(dh[3, :N].isnan().all()) and not bool(torch.isfinite(dh[T - 1, :N]).any())
+        assert bool((dh[T] == 7).all()) and bool((dh[:, N:] == 7).all())
+    if T > 100 and entry == "fwd":
+        assert bool(a[3, :N].isnan().all()) and bool((scales[[3, T - 1]] == 255).all())
+    assert bool((a[T] == 7).all()) and bool((a[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize("C", [96, 384])
+def test_mlp_of_the_fused_products_equals_that_of_the_separate_ones(C, monkeypatch):
+    """vil_mlp_act8 at a size whose products take the fused epilogues against the same block without them: y, and each gradient, to
+    12 half steps of the rms (as above: h and da are rounded in other places)"""
+    args = mlp_args(1000, C, 4 * C, torch.bfloat16, seed=3)
+    dy = data(3000, C, torch.bfloat16, 7).view(3, 1000, C)
+    out = []
+    for least in (1024, 1 << 40):
+        monkeypatch.setattr(act8, "_FUSE_MIN_T", least)
+        y = act8.vil_mlp_act8(*args)
+        out.append([y.detach(), *torch.autograd.grad(y, args, dy)])
+    for i, (a, b) in enumerate(zip(*out)):
+        a, b = a.double(), b.double()
+        assert float((a - b).norm()) <= 12 * 2.0 ** -8 * float(b.norm()), (i, float((a - b).norm() / b.norm()))
+
+
+def test_mlp_of_many_tokens_with_a_broadcast_gradient_an_expanded_or_a_strided_input():
+    """sizes that take the products with epilogues: rows that overlap are copied first, so the gradients are those of the copies"""
+    x, w1, b1, w2, b2 = mlp_args(1000, 96, 384, torch.bfloat16)
+    def grads(x, dy):
+        y = act8.vil_mlp_act8(x, w1, b1, w2, b2)
+        return [y.detach(), *torch.autograd.grad(y, (x, w1, b1, w2, b2), dy)]
+
+    row = data(1, 96, torch.bfloat16, 5)[0]
+    for dy in (row.expand(3, 1000, 96), row[0].expand(3, 1000, 96)):
+        for a, b in zip(grads(x, dy), grads(x, dy.contiguous())):
+            assert torch.equal(a, b)
+    dy = data(3000, 96, torch.bfloat16, 6).view(3, 1000, 96)
+    wide = torch.zeros(3, 1000, 104, device="cuda", dtype=torch.bfloat16)
+    wide[..., :96] = x.detach()
+    off = torch.zeros(3 * 1000 * 96 + 1, device="cuda", dtype=torch.bfloat16)
+    off[1:] = x.detach().view(-1)
+    want = grads(x, dy)
+    for a, b in zip(want, grads(wide[..., :96].requires_grad_(), dy)):
+        assert torch.equal(a, b)
+    for a, b in zip(want, grads(off[1:].view(3, 1000, 96).requires_grad_(), dy)):         # unaligned: the separate products
+        assert float((a - b).float().norm()) <= 12 * 2.0 ** -8 * float(a.float().norm())
+    same = x.detach()[:, :1].expand(3, 1000, 96).requires_grad_()
+    for a, b in zip(grads(same, dy), grads(same.detach().contiguous().requires_grad_(), dy)):
+        assert torch.equal(a, b)
+
+
+def test_mlp_refuses_parameters_that_do_not_fit():
+    x, w1, b1, w2, b2 = mlp_args(1000, 96, 384, torch.bfloat16)
+    for args in ((x, w1, b1[:-1], w2, b2), (x, w1, b1[None], w2, b2), (x, w1, b1, w2, b2[:1]), (x, w1, b1, w2, b1)):
+        with pytest.raises(ValueError):
+            act8.vil_mlp_act8(*args)
+    for i in range(1, 5):
+        args = [x, w1, b1, w2, b2]
+        args[i] = args[i].detach().cpu()
+        with pytest.raises(RuntimeError):
+            act8.vil_mlp_act8(*args)
+
+
+def test_mlp_of_many_tokens_captured_and_replayed():
+    x, w1, b1, w2, b2 = mlp_args(1000, 96, 384, torch.bfloat16)
+    dy = data(3000, 96, torch.bfloat16, 6).view(3, 1000, 96)
+
+    def step(v):
+        leaves = [t.detach().requires_grad_() for t in (v, w1, b1, w2, b2)]
+        y = act8.vil_mlp_act8(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    v = x.detach().clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(v)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(v)
+    for seed in range(3):
+        v.copy_(data(3000, 96, torch.bfloat16, seed).view(3, 1000, 96))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step(v)):
+            # (a product may be split another way in a capture: half a step of the rms)
+            assert float((a - b).float().norm()) <= 2.0 ** -8 * float(b.float().norm())

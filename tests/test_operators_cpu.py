@@ -80,6 +80,27 @@ def test_act8_c_entry_refuses():
     assert L.vil_gelu_act8_bwd(A16, A16, A16, BF16, 4, 64, 8, A16, None, None) == -2
 
 
+def test_act8_product_entries_refuse():
+    L = _lib.lib()
+    odd = ctypes.c_void_p(4100)
+    f = L.vil_gemm_gelu_act8_bf16
+    assert f(None, A16, None, A16, A16, A16, 2048, 96, 384, 96, 384, None) == -1
+    assert f(A16, A16, None, A16, A16, None, 2048, 96, 384, 96, 384, None) == -1
+    assert f(A16, A16, None, A16, A16, A16, 0, 96, 384, 96, 384, None) == -2
+    assert f(A16, A16, None, A16, A16, A16, 2048, 96, 384, 88, 384, None) == -2          # rows overlap
+    assert f(A16, A16, None, A16, A16, A16, 2048, 96, 384, 96, 376, None) == -2
+    assert f(A16, A16, None, A16, odd, A16, 2048, 96, 384, 96, 384, None) == -8
+    assert f(A16, A16, odd, A16, A16, A16, 2048, 96, 384, 96, 384, None) == -8
+    assert f(A16, A16, None, A16, A16, A16, 2048, 100, 384, 104, 384, None) == -10
+    assert f(A16, A16, None, A16, A16, A16, 2048, 96, 400, 96, 400, None) == -10
+    g = L.vil_gemm_dgelu_act8_bf16
+    assert g(A16, A16, None, A16, A16, A16, 2048, 96, 384, 96, 384, None) == -1
+    assert g(A16, A16, A16, A16, A16, A16, 2048, 96, 400, 96, 400, None) == -10
+    assert g(A16, A16, A16, ctypes.c_void_p(4097), A16, A16, 2048, 96, 384, 96, 384, None) == -8
+    assert g(A16, A16, A16, A16, A16, A16, 2048, 96, 384, 96, 376, None) == -2
+    assert g(A16, A16, A16, A16, A16, A16, 1 << 26, 96, 384, 96, 384, None) == -10           # 32-bit offsets
+
+
 def _args(**kw):
     a = dict(q=torch.zeros(2, 6, 3, 32), k=torch.zeros(2, 6, 3, 32), positions=torch.zeros(6, 2, dtype=torch.int32),
              inv_freq=torch.ones(16, dtype=torch.float64), sections=(8, 8))

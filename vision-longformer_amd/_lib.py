@@ -42,7 +42,8 @@ EXPORTS = ("vil_attn_abi_version", "vil_attn_strerror", "vil_attn_check", "vil_a
            "vil_optim_plan_bytes", "vil_optim_plan_build", "vil_optim_adamw_step", "vil_optim_qhm_step",
            "vil_optim_adamw_step_amp", "vil_optim_qhm_step_amp", "vil_attn_cw_set_shape", "vil_attn_cw_plan",
            "vil_qk_rope_workspace_bytes", "vil_qk_rope_fwd", "vil_qk_rope_bwd",
-           "vil_act8_pack", "vil_act8_unpack", "vil_gelu_act8_fwd", "vil_gelu_act8_bwd")
+           "vil_act8_pack", "vil_act8_unpack", "vil_gelu_act8_fwd", "vil_gelu_act8_bwd",
+           "vil_gemm_gelu_act8_bf16", "vil_gemm_dgelu_act8_bf16")
 
 
 class VilAttnDesc(ctypes.Structure):
@@ -240,6 +241,10 @@ def lib():
             L.vil_act8_unpack.argtypes = [vp, vp, i64, ci, vp, ci, vp]
             L.vil_gelu_act8_fwd.restype = ci
             L.vil_gelu_act8_fwd.argtypes = [vp, ci, i64, ci, i64, vp, vp, vp, vp]
+            L.vil_gemm_gelu_act8_bf16.restype = ci
+            L.vil_gemm_gelu_act8_bf16.argtypes = [vp] * 6 + [i64, ci, ci, i64, i64, vp]
+            L.vil_gemm_dgelu_act8_bf16.restype = ci
+            L.vil_gemm_dgelu_act8_bf16.argtypes = [vp] * 6 + [i64, ci, ci, i64, i64, vp]
             L.vil_gelu_act8_bwd.restype = ci
             L.vil_gelu_act8_bwd.argtypes = [vp, vp, vp, ci, i64, ci, i64, vp, vp, vp]
         if L.vil_attn_abi_version() != ABI_VERSION:

@@ -1,6 +1,7 @@
 """Activations held in 8 bits between the forward and the backward pass (libvilattn.so: vil_act8_* / vil_gelu_act8_*,
-csrc/vil_act8.hip): a general pack / unpack, the exact GELU whose backward pass reads its pre-activation from the packed
-form, and the MLP block built from them.
+csrc/vil_act8.hip; vil_gemm_*_act8_bf16, csrc/vil_gemm_fused.hip): a general pack / unpack, the exact GELU whose backward
+pass reads its pre-activation from the packed form, and the MLP block built from them, whose products carry both in their
+epilogues where that is faster.
 
 The reference's Mlp (src/models/msvit.py:17-34) keeps its input, fc1's output h and gelu(h) for the backward pass: 9 C values
 of 16 bits a token.  vil_mlp_act8 keeps the input and h in 8 bits (5 C of 1 1/32 bytes) and recomputes gelu from the packed h
@@ -148,6 +149,56 @@ def _linear(x2, w, b):
     return y if y is not None else F.linear(x2, w, b)
 
 
+# fc1 with the GELU and the packing in its epilogue, and fc2's input gradient with the GELU's backward on the packed form in its
+# epilogue (csrc/vil_gemm_fused.hip), against the library's product and vil_act8.hip's pass over its output; N = 4 K, device us, fused / separate:
+#   T x K     100352 x 96   100352 x 192   25088 x 384   25088 x 768   25088 x 1024   2048 x 192    1024 x 384    512 x 192
+#   forward      50 / 55       108 / 150       63 / 71      185 / 191      322 / 271    8.5 / 9.6    9.9 / 11.1    8.0 / 8.0
+#   backward     56 / 76       137 / 187       76 / 92      240 / 227      378 / 327     10 / 11     13.2 / 13.0   9.8 / 8.1
+# A longer K makes the product the larger part, and the library's is the faster one; few tokens are few tiles.
+_FUSE_MIN_T = 1024
+_FUSE_FWD_MAX_K, _FUSE_BWD_MAX_K = 768, 384
+
+
+def _aligned(*ts):
+    return all(t is None or (t.dtype == torch.bfloat16 and t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+                             and (t.dim() == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]))) for t in ts)
+
+
+def _fused(fn, T, K, N, rs, ts, outs):
+    try:
+        _lib.launch(outs[0].get_device(), fn, *[t.data_ptr() if t is not None else None for t in ts], *[t.data_ptr() for t in outs], T, K, N, rs, N)
+    except _lib.VilAttnError as e:
+        if e.code != _lib.VIL_E_BACKEND:
+            raise
+        return False
+    return True
+
+
+def _fused_fwd(x2, w, b):
+    """(gelu(h), h packed) of h = x2 @ w.T + b in one launch that never stores h; None where the separate ones are taken"""
+    T, K = x2.shape
+    N = w.shape[0]
+    if T < _FUSE_MIN_T or K > _FUSE_FWD_MAX_K or K % 32 or N % 128 or not (_aligned(x2, w, b) and w.is_contiguous()):
+        return None
+    a = x2.new_empty((T, N))
+    codes, scales = _empty(a)
+    if not _fused(_lib.lib().vil_gemm_gelu_act8_bf16, T, K, N, x2.stride(0), (x2, w, b), (a, codes, scales)):
+        return None
+    return a, Act8(codes, scales, a.shape, a.dtype)
+
+
+def _fused_bwd(dy2, w, packed):
+    """((dy2 @ w) * gelu'(v), gelu(v)), v the packed values, in one launch; None where the separate ones are taken"""
+    T, K = dy2.shape
+    N = w.shape[1]
+    if T < _FUSE_MIN_T or K > _FUSE_BWD_MAX_K or K % 32 or N % 128 or not (_aligned(dy2, w) and w.is_contiguous()):
+        return None
+    dh, a = dy2.new_empty((T, N)), dy2.new_empty((T, N))
+    if not _fused(_lib.lib().vil_gemm_dgelu_act8_bf16, T, K, N, dy2.stride(0), (dy2, w, packed.codes, packed.scales), (dh, a)):
+        return None
+    return dh, a
+
+
 def _weight_grad(dy2, x2, w, want_b):
     fused = _wgrad(dy2, x2, want_b)
     if fused is not None:
@@ -160,7 +211,8 @@ class _MlpAct8Fn(torch.autograd.Function):
     @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, w1, b1, w2, b2):
         x2 = _rows(x)
-        a, h8 = vil_gelu_act8_fwd(_linear(x2, w1, b1))
+        fused = _fused_fwd(x2, w1, b1)
+        a, h8 = fused if fused is not None else vil_gelu_act8_fwd(_linear(x2, w1, b1))
         y = _linear(a, w2, b2)
         x8 = vil_act8_pack(x2) if ctx.needs_input_grad[1] else None      # (x serves fc1's weight gradient alone)
         ctx.save_for_backward(*((x8.codes, x8.scales) if x8 is not None else (None, None)), h8.codes, h8.scales, w1, w2)
@@ -174,10 +226,14 @@ class _MlpAct8Fn(torch.autograd.Function):
         xc, xs, hc, hs, w1, w2 = ctx.saved_tensors
         shape, xshape, hshape, xt, ht, has_b1, has_b2 = ctx.was
         need = ctx.needs_input_grad
-        dy2 = dy.reshape(-1, dy.shape[-1])
-        da = _bwd_gemm(dy2, w2)
-        da = da if da is not None else dy2 @ w2
-        dh, a = vil_gelu_act8_bwd(Act8(hc, hs, hshape, ht), da, want_act=need[3])
+        dy2 = _rows(dy)                                                 # (a broadcast gradient's rows overlap: copied)
+        h8 = Act8(hc, hs, hshape, ht)
+        fused = _fused_bwd(dy2, w2, h8)
+        if fused is not None:
+            dh, a = fused
+        else:
+            da = _bwd_gemm(dy2, w2)
+            dh, a = vil_gelu_act8_bwd(h8, da if da is not None else dy2 @ w2, want_act=need[3])
         dx = dw1 = db1 = dw2 = db2 = None
         if need[3]:
             dw2, db2 = _weight_grad(dy2, a, w2, has_b2 and need[4])
@@ -205,5 +261,9 @@ def vil_mlp_act8(x, w1, b1, w2, b2):
         raise ValueError(f"vil_mlp_act8: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
     if not (w1.dtype == w2.dtype == x.dtype) or any(b is not None and b.dtype != x.dtype for b in (b1, b2)):
         raise TypeError(f"vil_mlp_act8: x is {x.dtype}, the parameters are {w1.dtype}, {w2.dtype}")
+    if any(b is not None and b.shape != w.shape[:1] for b, w in ((b1, w1), (b2, w2))):
+        raise ValueError(f"vil_mlp_act8: biases {[tuple(b.shape) for b in (b1, b2) if b is not None]} of weights {tuple(w1.shape)}, {tuple(w2.shape)}")
+    if any(p is not None and p.device != x.device for p in (w1, b1, w2, b2)):
+        raise RuntimeError(f"vil_mlp_act8: x is on {x.device}, a parameter is not")
     with torch.autocast("cuda", enabled=False):
         return _MlpAct8Fn.apply(x, w1, b1, w2, b2)

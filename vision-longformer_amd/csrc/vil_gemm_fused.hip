@@ -15,12 +15,14 @@
 // row-major [k][n] LDS image; B operand = dY rows (two 8-byte reads per fragment: the transposed read delivers k in the
 // order {4g + e, 16 + 4g + e}, so the other operand is read in that order too).  K streams in 64-deep blocks through a
 // two-slot LDS ring filled by LDS-DMA (the XOR-swizzled image of vil_attn_dense.hip).  Rows t >= T and k >= K read as
-// zeros through the bounded descriptors (w); a dY chunk beyond K in the last block is finite data of the next row
-// times those zeros.
+// zeros through the bounded descriptors; a dY chunk beyond K in the last block is requested past its descriptor's end, since
+// what stands there in memory is the next row, and a NaN of it times w's zeros would reach this one.
 #include "vil_mfma_common.h"
+#include "vil_act8.h"
 
 struct DgParams {
   const void* dy; const void* w; const void* h; void* dh;
+  const void* codes; const void* scales; void* a;      // PACK: the packed h instead of h; a = gelu of its values, dh's row stride
   int T, K, N;
   int dy_rs, h_rs, dh_rs;      // row strides, elements
   int nn_tiles;                // N / 128
@@ -81,8 +83,20 @@ __device__ __forceinline__ void gf_tiles(int ntiles, int& first, int& end, int& 
   first = lo + (int)(blockIdx.x >> 3);
 }
 
+template <typename C2> __device__ __forceinline__ void gf_store8(void* base, unsigned byte_off, const C2& v) {
+  asm volatile("global_store_dwordx2 %0, %1, %2" ::"v"(byte_off), "v"(v), "s"(base) : "memory");
+}
+__device__ __forceinline__ void gf_store1(void* base, unsigned byte_off, unsigned v) {
+  asm volatile("global_store_byte %0, %1, %2" ::"v"(byte_off), "v"(v), "s"(base) : "memory");
+}
+
 // DGELU = false: the plain input gradient dx = dy . w (vil_gemm_tile_bf16 op 1): no h loads, no derivative.
-template <bool DGELU>
+// PACK: h comes in its 8-bit form (vil_act8.h) and a = gelu(its values) is written beside dh: the operand of the next weight
+// gradient, which nothing kept.  A lane's eight features are a quarter of a block; the four lanes of a row (lg) read one scale.
+// All of a tile's codes (24 registers with the scales' pairs) are requested in front of the K loop and claimed before the first
+// store: half the bytes of h leave no reason for two batches.  Against the separate product and pass (T x K -> N, us): 100352 x 96
+// -> 384 56 / 76, 100352 x 192 -> 768 137 / 187, 25088 x 384 -> 1536 76 / 92; K = 768 is slower and left to the library.
+template <bool DGELU, bool PACK = false>
 __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
   typedef __bf16 T_;
   typedef typename V16<T_>::x8 X8;
@@ -102,13 +116,13 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
     const int drow = lane >> 3, dchunk = (lane & 7) ^ (((drow >> 1) & 3) << 1);
     auto issue = [&](int tl, int kb, int slot) {           // 32 one-kilobyte pieces of block kb of tile tl
       const int tile_t = tl / p.nn_tiles, tile_n = tl - tile_t * p.nn_tiles;
-      const int dy_v0 = (tile_t * 128 + drow) * (p.dy_rs * 2) + dchunk * 16 + kb * 128;
+      const unsigned dy_v0 = kb * 64 + dchunk * 8 < p.K ? (unsigned)((tile_t * 128 + drow) * (p.dy_rs * 2) + dchunk * 16 + kb * 128) : 1u << 31;
       const int w_v0 = (kb * 64 + drow) * (p.N * 2) + tile_n * 256 + dchunk * 16;
       char* base = smem + slot * GF_SLOT;
 #pragma unroll
       for (int pc = 0; pc < 16; ++pc)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(dyr, (__attribute__((address_space(3))) void*)(base + pc * 1024), 16,
-                                                 dy_v0 + pc * 8 * (p.dy_rs * 2), 0, 0, 0);
+                                                 (int)(dy_v0 + (unsigned)(pc * 8 * (p.dy_rs * 2))), 0, 0, 0);
 #pragma unroll
       for (int q = 0; q < 16; ++q)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(base + (16 + q) * 1024), 16,
@@ -154,11 +168,22 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
       return *(const X8*)((const char*)hb + (unsigned)(t * p.h_rs + n0 + wn * 64 + pr * 32 + lg * 8) * 2u);
     };
     X8 ha[2][2];
-    if (DGELU) {
+    a8_codes8 hc[4][2];
+    unsigned hs[4];
+    if (DGELU && !PACK) {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr) ha[tt][pr] = load_h(tt, pr);
+    }
+    if (PACK) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const unsigned t = (unsigned)min(t0 + wt * 64 + tt * 16 + lj, p.T - 1), n = (unsigned)(n0 + wn * 64);
+        hs[tt] = *(const uint16_t*)((const char*)p.scales + (t * (unsigned)p.N + n) / 32);     // blocks n / 32 (even) and the next
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) hc[tt][pr] = *(const a8_codes8*)((const char*)p.codes + (t * (unsigned)p.N + n + pr * 32 + lg * 8));
+      }
     }
     f32x4 acc[4][4];
 #pragma unroll
@@ -211,6 +236,33 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
     // Order: request h of token tiles 2, 3 -> results of tiles 0, 1 (held) -> claim the four late loads at once -> stores
     // of tiles 0, 1 -> tiles 2, 3.  No wait hipcc places for a load may follow a store of this tile: its counted
     // waits count the untracked stores too and would drain them.
+    if (PACK) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) asm volatile("" : "+v"(hc[tt][0]), "+v"(hc[tt][1]), "+v"(hs[tt]));
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const int t = t0 + wt * 64 + tt * 16 + lj;
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr) {
+          float v[8];
+          X8 o8, a8;
+          a8_decode(hc[tt][pr], (hs[tt] >> (8 * pr)) & 255, v);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            float hx, s;
+            a8_gelu<false>(v[r], hx, s);
+            o8[r] = (T_)a8_slope(acc[2 * pr + (r >> 2)][tt][r & 3], v[r], hx, s);
+            a8[r] = (T_)a8_act(v[r], hx, s);
+          }
+          if (t < p.T) {
+            const unsigned o = (unsigned)(t * p.dh_rs + n0 + wn * 64 + pr * 32 + lg * 8) * 2u;
+            gf_store16(ob, o, o8);
+            gf_store16(p.a, o, a8);
+          }
+        }
+      }
+      continue;
+    }
     X8 hl[2][2];
     if (DGELU) {
 #pragma unroll
@@ -261,6 +313,7 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
 // 16 nt + j of a wave's 64-row half holds weight row 32 (nt / 2) + 8 (j / 4) + 4 (nt % 2) + j % 4.
 struct FgParams {
   const void* x; const void* w; const void* bias; void* h; void* a;
+  void* codes; void* scales;   // PACK: h in its 8-bit form (vil_act8.h) instead of h
   int T, K, N;
   int x_rs, o_rs;              // row strides, elements
   int nn_tiles;                // N / 128
@@ -279,8 +332,10 @@ __device__ __forceinline__ float gelu_fwd(float x) {
   return x * (x < 0.f ? hc : 1.0f - hc);
 }
 
-// GELU = false: the plain forward h = x W^T + b (vil_gemm_tile_bf16 op 0): one output.
-template <bool GELU>
+// GELU = false: the plain forward h = x W^T + b (vil_gemm_tile_bf16 op 0): one output.  PACK: the rounded h is packed to 8 bits in
+// place of its store; the maximum of a block of 32 features is that of a row's four lanes, 16 apart.  Against the separate product and
+// pass (us): 100352 x 96 -> 384 50 / 55, 100352 x 192 -> 768 108 / 150, 25088 x 384 -> 1536 63 / 71.
+template <bool GELU, bool PACK = false>
 __global__ __launch_bounds__(GF_THREADS, 3) void k_fwd_gelu(FgParams p) {
   typedef __bf16 T_;
   typedef typename V16<T_>::x8 X8;
@@ -386,6 +441,26 @@ __global__ __launch_bounds__(GF_THREADS, 3) void k_fwd_gelu(FgParams p) {
           o8[r] = (T_)(acc[2 * pr][tt][r] + (float)bias8[pr][r]);
           o8[4 + r] = (T_)(acc[2 * pr + 1][tt][r] + (float)bias8[pr][4 + r]);
         }
+        if (PACK) {
+          uint32_t m = a8_lane_max<T_>(o8);
+          m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+          m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+          const int e = a8_exponent(m);
+          float v[8], act[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = (float)o8[r];
+          const a8_codes8 c = a8_encode<T_>(v, e);
+          a8_act8<false>(v, e, act);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) a8[r] = (T_)act[r];
+          if (t < p.T) {
+            const unsigned at = (unsigned)t * (unsigned)p.N + n0 + wn * 64 + pr * 32;
+            gf_store8(p.codes, at + lg * 8, c);
+            if (lg == 0) gf_store1(p.scales, at / 32, (unsigned)e);
+            gf_store16(ab, (unsigned)(t * p.o_rs + n0 + wn * 64 + pr * 32 + lg * 8) * 2u, a8);
+          }
+          continue;
+        }
         if (GELU) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) a8[r] = (T_)gelu_fwd((float)o8[r]);       // GELU of the rounded pre-activation
@@ -487,5 +562,54 @@ extern "C" int vil_gemm_tile_bf16(int op, const void* in, const void* w, const v
     if (int he = vil_ensure_dyn_lds((const void*)k_dgrad_dgelu<false>, lds)) return he;
     k_dgrad_dgelu<false><<<dim3(grid), dim3(GF_THREADS), lds, (hipStream_t)stream>>>(p);
   }
+  return (int)hipGetLastError();
+}
+
+// vil_gemm_gelu_bf16 with h in its 8-bit form (vil_act8.h): a[T][N] = gelu(h), codes int8 (T, N), scales uint8 (T, N / 32) of the rounded
+// bf16 h = x . w^T + bias.
+extern "C" int vil_gemm_gelu_act8_bf16(const void* x, const void* w, const void* bias, void* a, void* codes, void* scales, int64_t T,
+                                       int K, int N, int64_t x_row_stride, int64_t a_row_stride, void* stream) {
+  if (!x || !w || !a || !codes || !scales) return VIL_E_NULL;
+  if (T <= 0 || K <= 0 || N <= 0) return VIL_E_SHAPE;
+  if ((K & 31) || (N & 127)) return VIL_E_BACKEND;
+  if ((x_row_stride & 7) || (a_row_stride & 7) || (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & 15) || ((uintptr_t)codes & 7) ||
+      (bias && ((uintptr_t)bias & 15))) return VIL_E_ALIGN;
+  if (x_row_stride < K || a_row_stride < N) return VIL_E_SHAPE;
+  if ((T + 128) * x_row_stride * 2 >= (1ll << 31) || (int64_t)K * N * 2 >= (1ll << 31) || T * (N / 128) >= (1ll << 30)) return VIL_E_BACKEND;
+  if ((T + 128) * a_row_stride * 2 >= (1ll << 32)) return VIL_E_BACKEND;        // 32-bit byte offsets of the stores
+  FgParams p;
+  p.x = x; p.w = w; p.bias = bias; p.h = nullptr; p.a = a; p.codes = codes; p.scales = scales;
+  p.T = (int)T; p.K = K; p.N = N;
+  p.x_rs = (int)x_row_stride; p.o_rs = (int)a_row_stride;
+  p.nn_tiles = N / 128;
+  p.ntiles = (int)(((T + 127) / 128) * p.nn_tiles);
+  const size_t lds = 2 * GF_SLOT;
+  const unsigned grid = (unsigned)vil_persistent_grid(3, GF_THREADS / 64, lds, 1, (int64_t)p.ntiles * (GF_THREADS / 64));
+  if (int he = vil_ensure_dyn_lds((const void*)k_fwd_gelu<true, true>, lds)) return he;
+  k_fwd_gelu<true, true><<<dim3(grid), dim3(GF_THREADS), lds, (hipStream_t)stream>>>(p);
+  return (int)hipGetLastError();
+}
+
+// vil_gemm_dgelu_bf16 with h in its 8-bit form: with v = the values it stands for, dh = (dy . w) * gelu'(v) and a = gelu(v).
+extern "C" int vil_gemm_dgelu_act8_bf16(const void* dy, const void* w, const void* codes, const void* scales, void* dh, void* a, int64_t T,
+                                        int K, int N, int64_t dy_row_stride, int64_t out_row_stride, void* stream) {
+  if (!dy || !w || !codes || !scales || !dh || !a) return VIL_E_NULL;
+  if (T <= 0 || K <= 0 || N <= 0) return VIL_E_SHAPE;
+  if ((K & 31) || (N & 127)) return VIL_E_BACKEND;
+  if ((dy_row_stride & 7) || (out_row_stride & 7) || (((uintptr_t)dy | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)a) & 15) ||
+      ((uintptr_t)codes & 7) || ((uintptr_t)scales & 1)) return VIL_E_ALIGN;
+  if (dy_row_stride < K || out_row_stride < N) return VIL_E_SHAPE;
+  if ((T + 128) * dy_row_stride * 2 >= (1ll << 31) || (int64_t)K * N * 2 >= (1ll << 31) || T * (N / 128) >= (1ll << 30)) return VIL_E_BACKEND;
+  if ((T + 128) * out_row_stride * 2 >= (1ll << 32)) return VIL_E_BACKEND;
+  DgParams p;
+  p.dy = dy; p.w = w; p.h = nullptr; p.dh = dh; p.codes = codes; p.scales = scales; p.a = a;
+  p.T = (int)T; p.K = K; p.N = N;
+  p.dy_rs = (int)dy_row_stride; p.h_rs = 0; p.dh_rs = (int)out_row_stride;
+  p.nn_tiles = N / 128;
+  p.ntiles = (int)(((T + 127) / 128) * p.nn_tiles);
+  const size_t lds = 2 * GF_SLOT;
+  const unsigned grid = (unsigned)vil_persistent_grid(3, GF_THREADS / 64, lds, 1, (int64_t)p.ntiles * (GF_THREADS / 64));
+  if (int he = vil_ensure_dyn_lds((const void*)k_dgrad_dgelu<true, true>, lds)) return he;
+  k_dgrad_dgelu<true, true><<<dim3(grid), dim3(GF_THREADS), lds, (hipStream_t)stream>>>(p);
   return (int)hipGetLastError();
 }
