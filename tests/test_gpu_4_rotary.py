@@ -480,3 +480,24 @@ def test_same_tensor_twice_and_rows_behind_the_last():
     one, = torch.autograd.grad(a, x, torch.ones_like(a), retain_graph=True)
     two, = torch.autograd.grad((a, b), x, (torch.ones_like(a), torch.ones_like(b)))
     assert torch.equal(two, 2 * one) and torch.equal(buf, keep)
+
+
+@pytest.mark.parametrize("t", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,sections", [(10, (2,)), (48, (2,)), (48, (8, 8)), (64, (16, 16))])
+@pytest.mark.parametrize("scale", [-46, 46, 57])
+def test_norm_of_very_small_and_very_large_rows(scale, M, sections, t):
+    """rows of 10^-14 (eps = 0), 10^14 and 10^17: their squares fit fp32, and so does everything that the norm and its gradient
+    need in the order that the kernels take it"""
+    t = TYPES[t]
+    q, k, gq, gk, wq, wk = make(2, 33, 3, 3, M, t, False)
+    q, k = (v * 2.0 ** scale for v in (q, k))
+    pos, f = positions_of("grid", 2, 33, len(sections)), rotary.rotary_frequencies(sections, device="cuda")
+    q, k, wq, wk = (v.detach().requires_grad_() for v in (q, k, wq, wk))
+    y = rotary.vil_qk_norm_rope(q, k, wq, wk, positions=pos, inv_freq=f, sections=sections, eps=0.0)
+    grads = torch.autograd.grad(y, (q, k, wq, wk), (gq, gk))
+    cos, sin = angles(pos, f, sections)
+    for i, (x, w, g) in enumerate(((q, wq, gq), (k, wk, gk))):
+        ref = reference(x.detach().double(), w.detach().double(), g.double(), cos, sin, "half", True, 0.0)
+        check("y%d" % i, y[i].detach(), *ref["y"], t)
+        check("dx%d" % i, grads[i], *ref["dx"], t)
+        check("dw%d" % i, grads[2 + i], *ref["dw"], torch.float32)

@@ -475,7 +475,7 @@ __global__ __launch_bounds__(RO_THREADS, 4) void k_rope_norm_bwd(RoParams p) {
         }
         if (LPR > 2 && !u.on) s1 = s2 = 0.f;
         const float r = __builtin_amdgcn_rsqf(fmaf(ro_lane_sum<LPR>(s1), p.inv_m, p.eps));
-        const float m = r * r * r * (ro_lane_sum<LPR>(s2) * p.inv_m);
+        const float m = r * (r * (r * (ro_lane_sum<LPR>(s2) * p.inv_m)));    // (r^3 alone leaves fp32 past |x| = 10^12 and 10^-13)
         if (ok && u.on) {
           char* y = (char*)S.y + (seg * S.y_sb + t0 * S.y_st) * SZ;
           const unsigned yo = __umul24(tt, yt) + __umul24(h, yh);
