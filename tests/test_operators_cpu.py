@@ -101,6 +101,16 @@ def test_act8_product_entries_refuse():
     assert g(A16, A16, A16, A16, A16, A16, 1 << 26, 96, 384, 96, 384, None) == -10           # 32-bit offsets
 
 
+def test_a_packed_form_of_another_row_length_is_refused():
+    """(2, 96) in codes of (4, 48) has as many values, but six scales instead of eight"""
+    codes, scales = torch.zeros(2, 96, dtype=torch.int8), torch.zeros(2, 3, dtype=torch.uint8)
+    for shape in ((4, 48), (192,), ()):
+        with pytest.raises(ValueError):
+            act8.vil_act8_unpack(act8.Act8(codes, scales, shape, torch.float32))
+    with pytest.raises(RuntimeError):
+        act8.vil_act8_unpack(act8.Act8(codes, scales, (2, 96), torch.float32))
+
+
 def _args(**kw):
     a = dict(q=torch.zeros(2, 6, 3, 32), k=torch.zeros(2, 6, 3, 32), positions=torch.zeros(6, 2, dtype=torch.int32),
              inv_freq=torch.ones(16, dtype=torch.float64), sections=(8, 8))

@@ -49,7 +49,7 @@ def _check(x, name):
 def _check_packed(p, name):
     c, e = p.codes, p.scales
     if (c.dtype != torch.int8 or e.dtype != torch.uint8 or c.dim() != 2 or tuple(e.shape) != (c.shape[0], -(-c.shape[1] // BLOCK))
-            or c.numel() != p.shape.numel() or not c.is_contiguous() or not e.is_contiguous()):
+            or not p.shape or c.shape[1] != p.shape[-1] or c.numel() != p.shape.numel() or not c.is_contiguous() or not e.is_contiguous()):
         raise ValueError(f"{name}: codes {tuple(c.shape)} {c.dtype} and scales {tuple(e.shape)} {e.dtype} of {tuple(p.shape)}")
     if not c.is_cuda or e.device != c.device:
         raise RuntimeError(f"{name} needs device tensors: the product path is the HIP kernels (libvilattn.so); there is no CPU "
