@@ -480,3 +480,18 @@ def test_mlp_of_many_tokens_captured_and_replayed():
         for a, b in zip(got, step(v)):
             # (a product may be split another way in a capture: half a step of the rms)
             assert float((a - b).float().norm()) <= 2.0 ** -8 * float(b.float().norm())
+
+
+@pytest.mark.parametrize("K", [96, 160])
+def test_a_row_that_is_not_finite_stays_in_its_row_of_the_input_gradient(K):
+    """K % 64 = 32: the second half of the last block is no row's (the product with h in 16 bits, which shares the loader)"""
+    from vision_longformer_amd import linear
+    T, N, t = 1100, 384, torch.bfloat16
+    dy, w, h = data(T, K, t), data(K, N, t, 1), data(T, N, t, 2)
+    want = linear._dgrad_dgelu(dy, w, h)
+    bad = dy.clone()
+    bad[700, 3], bad[T - 1, 0] = float("nan"), float("inf")
+    got = linear._dgrad_dgelu(bad, w, h)
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[700] = keep[T - 1] = False
+    assert torch.equal(got[keep], want[keep]) and bool(got[700].isnan().all()) and bool(torch.isfinite(want).all())
