@@ -1,0 +1,23 @@
+"""CPU: vil_rotary_attention_qkv -- what it refuses before anything touches the device."""
+import pytest
+import torch
+
+from vision_longformer_amd import ops, rotary
+
+
+def args(nx=14, ny=14, nglo=1, H=2, M=64, **kw):
+    """a packed projection with norm and rotation; table, g2l, g2g of the sliding-chunk layers unless given"""
+    w = kw.get("w")
+    side = 4 * w - 1 if w is not None else 2 * max(nx, ny) - 1
+    a = dict(qkv=torch.zeros(2, nglo + nx * ny, 3 * H * M, dtype=torch.bfloat16), bias_table=torch.zeros(side * side, H),
+             g2l_bias=torch.zeros(2, H, nglo), g2g_bias=torch.zeros(H, nglo, nglo), nx=nx, ny=ny, nglo=nglo, num_heads=H, norm=True)
+    a.update(rotary.GridTurn(M).of(nx, ny, nglo, torch.device("cpu")))
+    return {**a, **kw}
+
+
+def test_windows_have_no_dense_kernels():
+    """backend "dense" attends to all tokens and reads a (2 nx - 1)(2 ny - 1) table: with a window it has neither"""
+    with pytest.raises(ValueError, match="dense"):
+        ops.vil_rotary_attention_qkv(**args(w=4, backend="dense"))
+    with pytest.raises(RuntimeError, match="device tensors"):
+        ops.vil_rotary_attention_qkv(**args(w=4))

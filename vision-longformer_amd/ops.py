@@ -595,6 +595,9 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
         raise ValueError("vil_rotary_attention_qkv: weights without the norm")
     if not norm and positions is None:
         raise ValueError("vil_rotary_attention_qkv: neither a norm nor positions: vil_full_attention_qkv or vil_dense_attention")
+    backend = backend or DEFAULT_BACKEND
+    if w is not None and backend == "dense":
+        raise ValueError("vil_rotary_attention_qkv: the dense kernel family attends to all tokens and knows no window")
     _check_dev(qkv, "vil_rotary_attention_qkv")
     qkv = _last_contig(qkv)
     if not 0 <= nglo <= FULL_MAX_G or (w is not None and nglo == 0):
@@ -602,7 +605,6 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
     if nglo == 0:
         g2l_bias = g2g_bias = None
     C = qkv.shape[-1] // 3
-    backend = backend or DEFAULT_BACKEND
     if w is not None:
         if exact not in (0, 1, -1) or (exact == 1 and mode != 0):
             raise ValueError("longsc exact should be in [0,1,-1]!")
