@@ -21,3 +21,23 @@ def test_windows_have_no_dense_kernels():
         ops.vil_rotary_attention_qkv(**args(w=4, backend="dense"))
     with pytest.raises(RuntimeError, match="device tensors"):
         ops.vil_rotary_attention_qkv(**args(w=4))
+
+
+@pytest.mark.parametrize("w", [None, 4])
+@pytest.mark.parametrize("which,shape", [("bias_table", (26 * 26, 2)), ("bias_table", (27 * 27, 1)), ("bias_table", (15, 15, 2)),
+                                         ("g2l_bias", (2, 2)), ("g2l_bias", (1, 2, 1)), ("g2g_bias", (2, 2, 1)), ("g2g_bias", (1, 1, 1))])
+def test_biases_of_another_shape_are_refused(w, which, shape):
+    """the kernels read them by address"""
+    with pytest.raises(ValueError, match=which):
+        ops.vil_rotary_attention_qkv(**args(w=w, **{which: torch.zeros(shape)}))
+    with pytest.raises(RuntimeError, match="device tensors"):
+        ops.vil_rotary_attention_qkv(**args(w=w, **{which: None}))
+
+
+@pytest.mark.parametrize("w", [None, 4])
+@pytest.mark.parametrize("which", ["bias_table", "g2l_bias", "g2g_bias"])
+def test_biases_on_another_device_are_refused(w, which):
+    a = args(w=w)
+    a[which] = a[which].to("meta")
+    with pytest.raises(RuntimeError, match=which + " on meta"):
+        ops.vil_rotary_attention_qkv(**a)

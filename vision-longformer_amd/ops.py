@@ -577,6 +577,18 @@ class _VilRotaryAttention(torch.autograd.Function):
                 dg2g.to(gdt) if dg2g is not None else None, dwq, dwk, None, None, None, None, None)
 
 
+def _check_bias(name, qkv, num_heads, nglo, sides, table, g2l, g2g):
+    """The kernels read sides[0] x sides[1] rows of the table and every global token's bias by address, on qkv's device."""
+    for t, what, shape in ((table, "bias_table", (sides[0] * sides[1], num_heads)), (g2l, "g2l_bias", (2, num_heads, nglo)),
+                           (g2g, "g2g_bias", (num_heads, nglo, nglo))):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name}: {what} of {shape} wanted; got {tuple(t.shape)}")
+        if t.device != qkv.device:
+            raise RuntimeError(f"{name}: qkv is on {qkv.device}, {what} on {t.device}")
+
+
 def _heads(t, H):
     return t.unflatten(-1, (H, t.shape[-1] // H))
 
@@ -598,7 +610,6 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
     backend = backend or DEFAULT_BACKEND
     if w is not None and backend == "dense":
         raise ValueError("vil_rotary_attention_qkv: the dense kernel family attends to all tokens and knows no window")
-    _check_dev(qkv, "vil_rotary_attention_qkv")
     qkv = _last_contig(qkv)
     if not 0 <= nglo <= FULL_MAX_G or (w is not None and nglo == 0):
         raise ValueError(f"vil_rotary_attention_qkv: nglo {nglo}")
@@ -608,6 +619,7 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
     if w is not None:
         if exact not in (0, 1, -1) or (exact == 1 and mode != 0):
             raise ValueError("longsc exact should be in [0,1,-1]!")
+        _check_bias("vil_rotary_attention_qkv", qkv, num_heads, nglo, (4 * int(w) - 1,) * 2, bias_table, g2l_bias, g2g_bias)
         cfg = _cfg(C, nx, ny, w, nglo, num_heads, mode, exact, scale)
         if mode_dev is not None:
             assert mode > 0 and mode_dev.dtype == torch.int32 and mode_dev.is_cuda
@@ -616,13 +628,15 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
         dense = (backend in ("auto", "dense") and dense_family_supported(qkv, nx, ny, nglo, num_heads)
                  and (bias_table is None or bias_table.shape[0] == (2 * int(nx) - 1) * (2 * int(ny) - 1)))
         if backend == "dense" and not dense:
+            _check_dev(qkv, "vil_rotary_attention_qkv")
             raise RuntimeError("vil_rotary_attention_qkv: the dense kernel family does not take this problem")
         side = 2 * max(int(nx), int(ny)) - 1
-        if not dense and bias_table is not None and bias_table.shape[0] != side * side:
-            raise ValueError(f"vil_rotary_attention_qkv: a bias table of {side} x {side} rows wanted")
+        _check_bias("vil_rotary_attention_qkv", qkv, num_heads, nglo, (2 * int(nx) - 1, 2 * int(ny) - 1) if dense else (side, side),
+                    bias_table, g2l_bias, g2g_bias)
         backend = "dense" if dense else backend
         cfg = _cfg(C, nx, ny, max(int(nx), int(ny)), nglo, num_heads, -1, 0, scale,
                    bias_side=side if bias_table is not None and not dense else 0)
+    _check_dev(qkv, "vil_rotary_attention_qkv")
     sections = tuple(int(n) for n in sections) if sections is not None else None
     return _VilRotaryAttention.apply(qkv, bias_table, g2l_bias, g2g_bias, q_weight, k_weight, positions, inv_freq, cfg,
                                      (sections, layout, bool(norm), float(eps)), backend)
