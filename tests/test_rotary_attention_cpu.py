@@ -41,3 +41,11 @@ def test_biases_on_another_device_are_refused(w, which):
     a[which] = a[which].to("meta")
     with pytest.raises(RuntimeError, match=which + " on meta"):
         ops.vil_rotary_attention_qkv(**a)
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan")])
+def test_eps_is_checked_like_vil_qk_norm_rope_s(eps):
+    """a negative one gives NaN where mean(x^2) is smaller"""
+    for f in (lambda: ops.vil_rotary_attention_qkv(**args(w=4, eps=eps)), lambda: rotary.vil_qk_norm_rope(torch.zeros(1, 1, 1, 8), eps=eps)):
+        with pytest.raises(ValueError, match="eps"):
+            f()

@@ -607,6 +607,8 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
         raise ValueError("vil_rotary_attention_qkv: weights without the norm")
     if not norm and positions is None:
         raise ValueError("vil_rotary_attention_qkv: neither a norm nor positions: vil_full_attention_qkv or vil_dense_attention")
+    if not eps >= 0:
+        raise ValueError(f"vil_rotary_attention_qkv: eps {eps}")
     backend = backend or DEFAULT_BACKEND
     if w is not None and backend == "dense":
         raise ValueError("vil_rotary_attention_qkv: the dense kernel family attends to all tokens and knows no window")
