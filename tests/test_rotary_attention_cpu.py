@@ -49,3 +49,33 @@ def test_eps_is_checked_like_vil_qk_norm_rope_s(eps):
     for f in (lambda: ops.vil_rotary_attention_qkv(**args(w=4, eps=eps)), lambda: rotary.vil_qk_norm_rope(torch.zeros(1, 1, 1, 8), eps=eps)):
         with pytest.raises(ValueError, match="eps"):
             f()
+
+
+@pytest.mark.parametrize("w", [None, 4])
+def test_a_second_derivative_is_refused(w, monkeypatch):
+    """With the launches replaced, and an incoming gradient that requires none: under create_graph the gradients come back, and a
+    penalty on them next to another term raises instead of leaving the attention's part out."""
+    def empty_out(q, *rest):
+        return torch.zeros_like(q), torch.zeros(1), torch.zeros(1)
+
+    def no_grads(q, k, v, out, dout, lse, lse_g, tab, g2l, g2g, dq, dk, dv, cfg, backend):
+        for t in (dq, dk, dv):
+            t.zero_()
+        return tab, g2l, g2g
+
+    monkeypatch.setattr(ops, "_check_dev", lambda *a: None)
+    monkeypatch.setattr(rotary, "_check", lambda *a: None)
+    monkeypatch.setattr(rotary, "_PLANS", {})                   # (none of this test's layouts is kept as checked)
+    monkeypatch.setattr(rotary, "_bwd", lambda plan, desc, gq, gk, q, k, wq, wk, pos, f, dq, dk, need_wq, need_wk: (
+        dq.zero_(), dk.zero_(), torch.zeros_like(wq), torch.zeros_like(wk))[2:])
+    monkeypatch.setattr(rotary._lib, "launch", lambda *a: None)
+    monkeypatch.setattr(ops, "_full_fwd", empty_out)
+    monkeypatch.setattr(ops, "_full_bwd", no_grads)
+    a = args(w=w, q_weight=torch.ones(64, requires_grad=True), k_weight=torch.ones(64, requires_grad=True))
+    leaves = [a[n].requires_grad_() for n in ("qkv", "bias_table", "g2l_bias", "g2g_bias", "q_weight", "k_weight")]
+    out = ops.vil_rotary_attention_qkv(**a)
+    grads = torch.autograd.grad(out.float().sum(), leaves, create_graph=True)
+    for g, v in zip(grads, leaves):
+        assert g.shape == v.shape
+        with pytest.raises(RuntimeError):
+            (g.float().square().sum() + v.float().square().sum()).backward(retain_graph=True)

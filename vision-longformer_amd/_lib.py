@@ -4,6 +4,7 @@ The product path has no CPU fallback: if the shared library has not been built
 (``python -c 'import __graft_entry__ as g; g.build()'``) every entry point
 raises."""
 import ctypes
+import functools
 import os
 
 # torch must be imported BEFORE the library is dlopen'ed: PyTorch-ROCm ships its own
@@ -283,6 +284,22 @@ def launch(index, fn, *args):
             code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if code != 0:
         check(code)
+
+
+def first_derivative_only(backward):
+    """For a node's backward whose results have no derivative here.  Under create_graph they come back with a graph that raises
+    where it is used: torch's once_differentiable does so only if the incoming gradient requires one, but the results depend
+    on the node's inputs too."""
+    @functools.wraps(backward)
+    def first(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        out = out if isinstance(out, tuple) else (out,)
+        raising = torch._C._functions.DelayedError(b"libvilattn: the kernels give first derivatives only", len(out))
+        return raising(*[t.detach().requires_grad_() if t is not None else None for t in out])
+    return first
 
 
 def profile_begin(capacity=8192):

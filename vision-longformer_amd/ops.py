@@ -554,6 +554,7 @@ class _VilRotaryAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_lib.first_derivative_only
     def backward(ctx, dout):
         from . import rotary
         qkv, qk, out, lse, lse_g, tab, g2l_f, g2g_f, wq, wk, positions, inv_freq = ctx.saved_tensors
