@@ -1,0 +1,46 @@
+"""CPU: what the operators on q and k and the 8-bit ones do where a derivative is asked of them that the kernels do not give.  The
+launches are replaced (outputs hold whatever their memory holds); nothing touches a device."""
+import pytest
+import torch
+
+from vision_longformer_amd import _lib, rotary
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """names of the entry points that a test reaches"""
+    names = []
+    monkeypatch.setattr(_lib, "launch", lambda index, fn, *args: names.append(fn.__name__))
+    monkeypatch.setattr(rotary, "_check", lambda *a: None)
+    monkeypatch.setattr(rotary, "_PLANS", {})                   # (none of these layouts is kept as checked)
+    return names
+
+
+def qk(**kw):
+    q, k = torch.randn(1, 6, 2, 32, **kw), torch.randn(1, 6, 1, 32, **kw)
+    return q, k, dict(positions=rotary.grid_positions(2, 3), inv_freq=rotary.rotary_frequencies((8, 8)), sections=(8, 8))
+
+
+def test_norm_gradient_under_create_graph(launched):
+    """the incoming gradient requires none, the norm's gradient depends on q, k and the weights all the same"""
+    q, k, turn = qk(requires_grad=True)
+    w = torch.ones(32, requires_grad=True)
+    yq, yk = rotary.vil_qk_norm_rope(q, k, w, w, **turn)
+    grads = torch.autograd.grad(yq.sum() + yk.sum(), (q, k, w), create_graph=True)
+    for g, v in zip(grads, (q, k, w)):
+        assert g.shape == v.shape
+        with pytest.raises(RuntimeError):
+            (g.sum() + v.square().sum()).backward(retain_graph=True)
+    assert launched == ["vil_qk_rope_fwd", "vil_qk_rope_bwd"]
+
+
+def test_rotation_gradient_under_create_graph(launched):
+    """linear in q: nothing is left out where the incoming gradient is a constant, and where it is not, the call raises"""
+    q, _, turn = qk(requires_grad=True)
+    y = rotary.vil_rope(q, **turn)
+    g, = torch.autograd.grad(y.sum(), q, create_graph=True)
+    (g.sum() + q.square().sum()).backward(retain_graph=True)
+    assert torch.equal(q.grad, 2 * q.detach())
+    g, = torch.autograd.grad(y.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (g.sum() + q.square().sum()).backward()

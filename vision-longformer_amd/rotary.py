@@ -198,7 +198,11 @@ class _QKRope(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        return _QKRope.second(ctx, gq, gk) if torch.is_grad_enabled() else _QKRope.first(ctx, gq, gk)
+        if not torch.is_grad_enabled():
+            return _QKRope.first(ctx, gq, gk)
+        # under create_graph: the same values, and an error where a second derivative is asked of them.  The rotation alone is linear: its
+        # gradient depends on the incoming one only, the norm's on q and k too.
+        return (_QKRope.of_norm if ctx.plan.norm else _QKRope.of_rotation)(ctx, gq, gk)
 
     @staticmethod
     def first(ctx, gq, gk):
@@ -213,8 +217,8 @@ class _QKRope(torch.autograd.Function):
         dwq, dwk = _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need[2], need[3])
         return dq, dk, dwq, dwk, None, None, None
 
-    # under create_graph: the same values, and an error where a second derivative is asked of them
-    second = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, gq, gk: _QKRope.first(ctx, gq, gk)))
+    of_rotation = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, gq, gk: _QKRope.first(ctx, gq, gk)))
+    of_norm = staticmethod(_lib.first_derivative_only(lambda ctx, gq, gk: _QKRope.first(ctx, gq, gk)))
 
 
 def _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
