@@ -3,7 +3,7 @@ launches are replaced (outputs hold whatever their memory holds); nothing touche
 import pytest
 import torch
 
-from vision_longformer_amd import _lib, rotary
+from vision_longformer_amd import _lib, act8, rotary
 
 
 @pytest.fixture
@@ -12,6 +12,8 @@ def launched(monkeypatch):
     names = []
     monkeypatch.setattr(_lib, "launch", lambda index, fn, *args: names.append(fn.__name__))
     monkeypatch.setattr(rotary, "_check", lambda *a: None)
+    monkeypatch.setattr(act8, "_check", lambda *a: None)
+    monkeypatch.setattr(act8, "_check_packed", lambda *a: None)
     monkeypatch.setattr(rotary, "_PLANS", {})                   # (none of these layouts is kept as checked)
     return names
 
@@ -44,3 +46,18 @@ def test_rotation_gradient_under_create_graph(launched):
     g, = torch.autograd.grad(y.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         (g.sum() + q.square().sum()).backward()
+
+
+@pytest.mark.parametrize("op", ["gelu", "mlp"])
+def test_8_bit_gradients_under_create_graph(op, launched):
+    """the incoming gradient requires none, the GELU's slope depends on its input all the same"""
+    x = torch.randn(4, 32, requires_grad=True)
+    leaves = [x]
+    if op == "mlp":
+        leaves += [torch.randn(s, requires_grad=True) for s in ((64, 32), (64,), (32, 64), (32,))]
+    y = act8.vil_gelu_act8(x) if op == "gelu" else act8.vil_mlp_act8(*leaves)
+    for g, v in zip(torch.autograd.grad(y.sum(), leaves, create_graph=True), leaves):
+        assert g.shape == v.shape
+        with pytest.raises(RuntimeError):
+            (g.sum() + v.square().sum()).backward(retain_graph=True)
+    assert "vil_gelu_act8_fwd" in launched and "vil_gelu_act8_bwd" in launched

@@ -132,7 +132,7 @@ class _GeluAct8Fn(torch.autograd.Function):
         return a
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.first_derivative_only
     def backward(ctx, da):
         dh, _ = vil_gelu_act8_bwd(Act8(*ctx.saved_tensors, *ctx.was), da, want_act=False)
         return dh
@@ -221,7 +221,7 @@ class _MlpAct8Fn(torch.autograd.Function):
 
     @staticmethod
     @torch.amp.custom_bwd(device_type="cuda")
-    @torch.autograd.function.once_differentiable
+    @_lib.first_derivative_only
     def backward(ctx, dy):
         xc, xs, hc, hs, w1, w2 = ctx.saved_tensors
         shape, xshape, hshape, xt, ht, has_b1, has_b2 = ctx.was
