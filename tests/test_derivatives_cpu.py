@@ -2,6 +2,7 @@
 launches are replaced (outputs hold whatever their memory holds); nothing touches a device."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from vision_longformer_amd import _lib, act8, rotary
 
@@ -61,3 +62,36 @@ def test_8_bit_gradients_under_create_graph(op, launched):
         with pytest.raises(RuntimeError):
             (g.sum() + v.square().sum()).backward(retain_graph=True)
     assert "vil_gelu_act8_fwd" in launched and "vil_gelu_act8_bwd" in launched
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("norm", [True, False])
+def test_forward_mode_is_refused(norm, grad, launched):
+    """a dual tensor requires no gradient: its tangent must not be dropped for that"""
+    q, k, turn = qk()
+    fn = rotary.vil_qk_norm_rope if norm else rotary.vil_rope
+    with torch.set_grad_enabled(grad):
+        for at in (0, 1):
+            with forward_ad.dual_level():
+                dual = [q, k]
+                dual[at] = forward_ad.make_dual(dual[at], torch.ones_like(dual[at]))
+                with pytest.raises(NotImplementedError):
+                    fn(*dual, **turn)
+                if norm:
+                    with pytest.raises(NotImplementedError):
+                        fn(q, k, forward_ad.make_dual(torch.ones(32), torch.ones(32)), **turn)
+                assert fn(q, k, **turn)[at].shape == (q, k)[at].shape                # no tangent: an ordinary call
+        n = len(launched)
+        fn(q, k, **turn)
+        assert len(launched) == n + 1
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_a_traced_call_launches(norm, launched):
+    """a trace of a call without gradients records the node, not its empty outputs alone"""
+    q, k, turn = qk()
+    fn = rotary.vil_qk_norm_rope if norm else rotary.vil_rope
+    traced = torch.jit.trace(lambda q, k: fn(q, k, **turn), (q, k), check_trace=False)
+    n = len(launched)
+    yq, yk = traced(q, k)
+    assert launched[n:] == ["vil_qk_rope_fwd"] and yq.shape == q.shape and yk.shape == k.shape

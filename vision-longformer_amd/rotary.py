@@ -9,6 +9,7 @@ place.  There is no eager fallback: CPU tensors or a missing library raise."""
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -191,6 +192,9 @@ def _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need_wq,
 class _QKRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, inv_freq, plan):
+        """plan: a _Plan of tensors that _inputs has seen, or _inputs' name and options"""
+        if not isinstance(plan, _Plan):
+            plan, q, k, wq, wk, positions, inv_freq = _inputs(plan[0], q, k, wq, wk, positions, inv_freq, *plan[1:])
         ctx.plan = plan
         # without the norm the gradient is the rotation back: the inputs need not be kept
         ctx.save_for_backward(*((q, k) if plan.norm else (None, None)), wq, wk, positions, inv_freq)
@@ -241,6 +245,11 @@ def _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps
 
 
 def _apply(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
+    if forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None:
+        # a tangent, which only the node refuses; a trace, which records the node and not the launch, and whose sizes are no
+        # numbers outside it
+        yq, yk = _QKRope.apply(q, k, wq, wk, positions, inv_freq, (name, sections, layout, norm, eps))
+        return yq if k is None else (yq, yk)
     plan, *args = _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
         yq, yk = _QKRope.apply(*args, plan)
