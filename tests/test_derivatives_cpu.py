@@ -95,3 +95,18 @@ def test_a_traced_call_launches(norm, launched):
     n = len(launched)
     yq, yk = traced(q, k)
     assert launched[n:] == ["vil_qk_rope_fwd"] and yq.shape == q.shape and yk.shape == k.shape
+
+
+@pytest.mark.parametrize("fn", [lambda x: act8.vil_act8_unpack(act8.vil_act8_pack(x)), lambda x: act8.vil_gelu_act8_fwd(x)[0]])
+def test_calls_without_a_node_are_not_traced(fn, monkeypatch):
+    """(without `launched`: what refuses is the launch)"""
+    monkeypatch.setattr(act8, "_check", lambda *a: None)
+    monkeypatch.setattr(act8, "_check_packed", lambda *a: None)
+    with pytest.raises(RuntimeError, match="no launch"):
+        torch.jit.trace(fn, (torch.randn(4, 64),), check_trace=False)
+
+
+def test_a_traced_8_bit_gelu_launches(launched):
+    traced = torch.jit.trace(act8.vil_gelu_act8, (torch.randn(4, 64),), check_trace=False)
+    n = len(launched)
+    assert traced(torch.randn(4, 64)).shape == (4, 64) and launched[n:] == ["vil_gelu_act8_fwd"]

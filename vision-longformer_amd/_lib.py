@@ -277,6 +277,8 @@ def check(code):
 def launch(index, fn, *args):
     """fn(*args, stream) on device `index` and its current stream.  The two torch._C calls are what torch.cuda.current_device() and
     current_stream() end in, without the objects around them (8 of the 25 microseconds that a small call took)."""
+    if torch._C._get_tracing_state() is not None:        # (off inside an autograd node, which a trace records and runs again)
+        raise RuntimeError(f"{fn.__name__}: a trace would record the outputs' allocation and no launch")
     if torch._C._cuda_getDevice() == index:
         code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
