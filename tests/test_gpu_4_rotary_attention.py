@@ -39,3 +39,55 @@ def test_create_graph_gives_the_same_gradients_and_a_second_derivative_raises(w)
         assert torch.equal(x, y) or float((x - y).abs().max()) <= 2.0 ** -10 * float(x.abs().max())
         with pytest.raises(RuntimeError):
             (y.float().square().sum() + v.float().square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("how", ["wider_rows", "odd_wider_rows", "tokens_first", "one_image"])
+@pytest.mark.parametrize("w,t,M", [(7, "bf16", 64), (7, "fp32", 32), (None, "fp32", 64), (None, "bf16", 48), (None, "bf16", 64)])
+def test_a_projection_in_other_rows_takes_the_same_kernels(how, w, t, M):
+    """a slice of wider rows, or one whose tokens come first, on the matrix-core kernels (which take one stride for k and v) as the packed
+    projection itself: where the rotation's kernel is the same too, the same numbers in the same order, so equal outputs and gradients of
+    qkv and the norm's weights"""
+    H, N, t = 2, 197, TYPES[t]
+    a = args(w, t, M=M, H=H, B=1 if how == "one_image" else 2)
+    qkv, C3 = a["qkv"], 3 * H * M
+    if how == "tokens_first":
+        x = qkv.transpose(0, 1).contiguous().transpose(0, 1)
+    else:
+        wide = torch.zeros(qkv.shape[0], N, C3 + (5 if how == "odd_wider_rows" else 64), device="cuda", dtype=t)
+        wide[..., :C3] = qkv
+        x = wide[..., :C3]
+    assert x.stride(1) != C3 or how == "one_image"
+    dout = rnd(qkv.shape[0], N, H * M, seed=3, t=t)
+    backend = None if M == 64 and w is None and t == torch.bfloat16 else "mfma"        # (None: the dense family)
+    got = []
+    for v in (qkv, x):
+        leaves = [v.requires_grad_(), *(a[n].requires_grad_() for n in LEAVES[1:])]
+        out = ops.vil_rotary_attention_qkv(**{**a, "qkv": v}, backend=backend)
+        got.append((out.detach(), torch.autograd.grad(out, leaves, dout)))
+    (want, wg), (out, g) = got
+    if how == "odd_wider_rows":
+        # rows that 16-byte loads do not fit take the element-wise rotation, which adds a row's squares in another order: rotated values may
+        # round to the neighbouring number.  Either side is within the attention's bounds of the formulas (gpu_common: fp32 out 2e-5 +
+        # 1e-4, gradients 1e-4 + 1e-3; 16 bits 2e-2 + 5e-2, 6 % of the rms + 5 %), so the two are within twice those of each other.
+        low = t != torch.float32
+        for x, y, grad in ((out, want, False), *((g[i], wg[i], True) for i in range(6))):
+            x, y = x.double(), y.double()
+            s = float(y.square().mean().sqrt()) if grad else 1.0
+            lim = (0.06 * s if grad else 2e-2) + 5e-2 * y.abs() if low else (1e-4 * max(s, 1) if grad else 2e-5) + (1e-3 if grad else 1e-4) * y.abs()
+            assert bool(((x - y).abs() <= 2 * lim).all())
+        return
+    assert torch.equal(out, want)
+    for i in (0, 4, 5):
+        assert torch.equal(g[i], wg[i]), LEAVES[i]
+    for i in (1, 2, 3):                                          # (sums that may come in another order: as above)
+        assert float((g[i] - wg[i]).abs().max()) <= 2.0 ** -10 * float(wg[i].abs().max()), LEAVES[i]
+
+
+def test_rows_beside_a_sliced_projection_are_left_alone():
+    a = args(7, torch.bfloat16)
+    wide = rnd(2, 197, 400, seed=7, t=torch.bfloat16)
+    keep = wide.clone()
+    qkv = wide[..., 8:392].detach().requires_grad_()
+    out = ops.vil_rotary_attention_qkv(**{**a, "qkv": qkv}, backend="mfma")
+    g, = torch.autograd.grad(out, qkv, torch.ones_like(out))
+    assert torch.equal(wide, keep) and g.shape == qkv.shape and bool(torch.isfinite(g).all())

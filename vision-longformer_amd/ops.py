@@ -543,13 +543,18 @@ class _VilRotaryAttention(torch.autograd.Function):
         # the rotated q and k at the packed row's stride: the sliding-chunk kernels address k and v with one stride
         qk = torch.empty(B, N, C3, dtype=qkv.dtype, device=qkv.device)
         rotary._fwd(plan, q, k, wq, wk, positions, inv_freq, into=(_heads(qk[..., :C], H), _heads(qk[..., C:2 * C], H)))
+        # (a slice of wider rows, or tokens first: v goes beside them, or the matrix-core kernels would refuse the call)
+        v_beside = backend != "dense" and qkv.stride(1) != C3
+        if v_beside:
+            qk[..., 2 * C:] = qkv[..., 2 * C:]
+        views = (qk[..., :C], qk[..., C:2 * C], (qk if v_beside else qkv)[..., 2 * C:])
         tab, g2l_f, g2g_f = _f32c(table), _f32c(g2l), _f32c(g2g)
         if backend == "dense":
-            (out, lse), lse_g = _dense_fwd(qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:], tab, g2l_f, g2g_f, cfg), None
+            (out, lse), lse_g = _dense_fwd(*views, tab, g2l_f, g2g_f, cfg), None
         else:
-            out, lse, lse_g = _full_fwd(qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:], tab, g2l_f, g2g_f, cfg, backend)
+            out, lse, lse_g = _full_fwd(*views, tab, g2l_f, g2g_f, cfg, backend)
         ctx.save_for_backward(qkv, qk, out, lse, lse_g, tab, g2l_f, g2g_f, wq, wk, positions, inv_freq)
-        ctx.cfg, ctx.plan, ctx.backend = cfg, plan, backend
+        ctx.cfg, ctx.plan, ctx.backend, ctx.v_beside = cfg, plan, backend, v_beside
         ctx.dts = tuple(t.dtype if t is not None else None for t in (table, g2l, g2g))
         return out
 
@@ -564,7 +569,7 @@ class _VilRotaryAttention(torch.autograd.Function):
         dout = _last_contig(dout).to(qkv.dtype)
         dqkv = torch.empty_like(qkv)
         gq, gk = (torch.empty(B, N, C, dtype=qkv.dtype, device=qkv.device) for _ in range(2))
-        views = (qk[..., :C], qk[..., C:2 * C], qkv[..., 2 * C:])
+        views = (qk[..., :C], qk[..., C:2 * C], (qk if ctx.v_beside else qkv)[..., 2 * C:])
         if ctx.backend == "dense":
             dtab, dg2l, dg2g = _dense_bwd(*views, out, dout, lse, tab, g2l_f, g2g_f, gq, gk, dqkv[..., 2 * C:], cfg)
         else:
@@ -599,7 +604,7 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
                              sections=None, layout="half", norm=False, eps=1e-6):
     """vil_full_attention_qkv (w = the window) or vil_dense_attention (w = None) of a packed (B, N, 3C) projection whose q and k
     first pass vil_rope (norm=False) or vil_qk_norm_rope (norm=True; the weights may be None): one autograd node, v read in
-    place.  Arguments as those functions'; positions (N, axes) or (B, N, axes) cover the nglo global tokens, which come first."""
+    place (with w, from rows that follow each other; from others it is copied).  Arguments as those functions'; positions (N, axes) or (B, N, axes) cover the nglo global tokens, which come first."""
     if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads):
         raise ValueError(f"vil_rotary_attention_qkv: a packed projection of {num_heads} heads; got {tuple(qkv.shape)}")
     if qkv.shape[1] != nglo + nx * ny:
