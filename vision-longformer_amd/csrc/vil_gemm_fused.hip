@@ -15,8 +15,9 @@
 // row-major [k][n] LDS image; B operand = dY rows (two 8-byte reads per fragment: the transposed read delivers k in the
 // order {4g + e, 16 + 4g + e}, so the other operand is read in that order too).  K streams in 64-deep blocks through a
 // two-slot LDS ring filled by LDS-DMA (the XOR-swizzled image of vil_attn_dense.hip).  Rows t >= T and k >= K read as
-// zeros through the bounded descriptors; a dY chunk beyond K in the last block is requested past its descriptor's end, since
-// what stands there in memory is the next row, and a NaN of it times w's zeros would reach this one.
+// zeros through the bounded descriptors.  Where K % 64 is 32 no product reads the last block's second half (`nks`), which is the
+// next row's data: its dY chunks are requested past the descriptor's end, which fetches nothing (401408 x 96 -> 384: 159.4 us
+// against 161.8, in the 8-bit form 236.9 against 239.5).
 #include "vil_mfma_common.h"
 #include "vil_act8.h"
 
