@@ -76,6 +76,13 @@ template <typename X8> __device__ __forceinline__ void gf_store16(void* base, un
   // recognizer does not look into inline assembly)
   asm volatile("global_store_dwordx4 %0, %1, %2\n\ts_nop 1" ::"v"(byte_off), "v"(__builtin_bit_cast(gf_u32x4, v)), "s"(base) : "memory");
 }
+// the lane's number, made anew where it stands instead of carried through the tile loop (two instructions; k_dgrad_dgelu's 8-bit form
+// has no register for it: carried, it and two row indices were spilled, and a reload between a tile's stores drained them)
+__device__ __forceinline__ int gf_lane() {
+  unsigned zero = 0;
+  asm volatile("" : "+s"(zero));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
 __device__ __forceinline__ void gf_barrier() { asm volatile("s_barrier" ::: "memory"); }
 __device__ __forceinline__ void gf_tiles(int ntiles, int& first, int& end, int& stride) {
   const int per = (ntiles + 7) >> 3, lo = (int)(blockIdx.x & 7) * per;
@@ -93,10 +100,12 @@ __device__ __forceinline__ void gf_store1(void* base, unsigned byte_off, unsigne
 
 // DGELU = false: the plain input gradient dx = dy . w (vil_gemm_tile_bf16 op 1): no h loads, no derivative.
 // PACK: h comes in its 8-bit form (vil_act8.h) and a = gelu(its values) is written beside dh: the operand of the next weight
-// gradient, which nothing kept.  A lane's eight features are a quarter of a block; the four lanes of a row (lg) read one scale.
-// All of a tile's codes (24 registers with the scales' pairs) are requested in front of the K loop and claimed before the first
-// store: half the bytes of h leave no reason for two batches.  Against the separate product and pass (T x K -> N, us): 100352 x 96
-// -> 384 56 / 76, 100352 x 192 -> 768 137 / 187, 25088 x 384 -> 1536 76 / 92; K = 768 is slower and left to the library.
+// gradient, which nothing kept.  A lane's eight features are a quarter of a block; the four lanes of a row (lg) need one scale.
+// All of a tile's codes (16 registers) and scales (one: lane i has row i's pair, handed to its four lanes in the epilogue) are
+// requested in front of the K loop and claimed before the first store: half the bytes of h leave no reason for two batches.
+// 127 registers, no scratch.  128 is the limit: at 136 (a bound of 3 waves a SIMD) one workgroup less fits a CU, 103 us for 78 at
+// 25088 x 384 -> 1536.  Against the separate product and pass (T x K -> N, us): 100352 x 96 -> 384 55 / 76, 100352 x 192 -> 768
+// 138 / 187, 25088 x 384 -> 1536 78 / 92; K = 768 is slower (242 / 227) and left to the library.
 template <bool DGELU, bool PACK = false>
 __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
   typedef __bf16 T_;
@@ -170,7 +179,7 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
     };
     X8 ha[2][2];
     a8_codes8 hc[4][2];
-    unsigned hs[4];
+    unsigned hs = 0;
     if (DGELU && !PACK) {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
@@ -178,12 +187,14 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
         for (int pr = 0; pr < 2; ++pr) ha[tt][pr] = load_h(tt, pr);
     }
     if (PACK) {
+      const unsigned n = (unsigned)(n0 + wn * 64);
+      const int ln = gf_lane(), row = ln & 15, quarter = ln >> 4;
+      hs = *(const uint16_t*)((const char*)p.scales + ((unsigned)min(t0 + wt * 64 + ln, p.T - 1) * (unsigned)p.N + n) / 32);   // blocks n / 32 (even) and the next
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        const unsigned t = (unsigned)min(t0 + wt * 64 + tt * 16 + lj, p.T - 1), n = (unsigned)(n0 + wn * 64);
-        hs[tt] = *(const uint16_t*)((const char*)p.scales + (t * (unsigned)p.N + n) / 32);     // blocks n / 32 (even) and the next
+        const unsigned t = (unsigned)min(t0 + wt * 64 + tt * 16 + row, p.T - 1);
 #pragma unroll
-        for (int pr = 0; pr < 2; ++pr) hc[tt][pr] = *(const a8_codes8*)((const char*)p.codes + (t * (unsigned)p.N + n + pr * 32 + lg * 8));
+        for (int pr = 0; pr < 2; ++pr) hc[tt][pr] = *(const a8_codes8*)((const char*)p.codes + (t * (unsigned)p.N + n + pr * 32 + quarter * 8));
       }
     }
     f32x4 acc[4][4];
@@ -239,15 +250,18 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
     // waits count the untracked stores too and would drain them.
     if (PACK) {
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) asm volatile("" : "+v"(hc[tt][0]), "+v"(hc[tt][1]), "+v"(hs[tt]));
+      for (int tt = 0; tt < 4; ++tt) asm volatile("" : "+v"(hc[tt][0]), "+v"(hc[tt][1]));
+      asm volatile("" : "+v"(hs));
+      const int ln = gf_lane(), row = ln & 15, quarter = ln >> 4;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        const int t = t0 + wt * 64 + tt * 16 + lj;
+        const int t = t0 + wt * 64 + tt * 16 + row;
+        const unsigned e2 = (unsigned)__shfl((int)hs, tt * 16 + row, 64);
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr) {
           float v[8];
           X8 o8, a8;
-          a8_decode(hc[tt][pr], (hs[tt] >> (8 * pr)) & 255, v);
+          a8_decode(hc[tt][pr], (e2 >> (8 * pr)) & 255, v);
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             float hx, s;
@@ -256,7 +270,7 @@ __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
             a8[r] = (T_)a8_act(v[r], hx, s);
           }
           if (t < p.T) {
-            const unsigned o = (unsigned)(t * p.dh_rs + n0 + wn * 64 + pr * 32 + lg * 8) * 2u;
+            const unsigned o = (unsigned)(t * p.dh_rs + n0 + wn * 64 + pr * 32 + quarter * 8) * 2u;
             gf_store16(ob, o, o8);
             gf_store16(p.a, o, a8);
           }
