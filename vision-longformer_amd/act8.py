@@ -15,6 +15,7 @@ from .linear import _fwd_gemm, _bwd_gemm, _wgrad, _colsum
 
 _DT = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 BLOCK = 32
+_MAX_BLOCKS = (2 ** 24 - 1) * 128          # what one launch holds (csrc/vil_act8.hip)
 
 
 class Act8:
@@ -39,8 +40,9 @@ def _check(x, name):
         raise TypeError(f"{name} supports float32 / bfloat16 / float16; got {x.dtype}")
     if x.dim() < 1:
         raise ValueError(f"{name}: a tensor with at least one axis")
-    if x.shape[-1] >= 2 ** 31 or x.numel() > 2 ** 37:
-        raise ValueError(f"{name}: {tuple(x.shape)} is too large")
+    cols = x.shape[-1]
+    if cols >= 2 ** 31 or (cols and x.numel() // cols * -(-cols // BLOCK) > _MAX_BLOCKS):
+        raise ValueError(f"{name}: {tuple(x.shape)} is too large (2^31 blocks of {BLOCK} channels, filled or not)")
     if not x.is_cuda:
         raise RuntimeError(f"{name} needs device tensors: the product path is the HIP kernels (libvilattn.so); there is no CPU "
                            "fallback")

@@ -31,8 +31,7 @@ __device__ __forceinline__ A8At a8_at(int64_t lane, int64_t rows, int cols, int 
     w.n = w.row < rows ? 8 : 0;                            // (rows: the number of values)
     return w;
   }
-  if (rows * nb < ((int64_t)1 << 31)) w.row = (uint32_t)w.blk / (uint32_t)nb;
-  else w.row = w.blk / nb;
+  w.row = (uint32_t)w.blk / (uint32_t)nb;                  // (blocks: under 2^31, a8_check)
   w.c = (int)(w.blk - w.row * nb) * A8_BLOCK + (int)(lane & 3) * 8;
   w.n = w.row < rows ? cols - w.c : 0;
   w.n = w.n < 0 ? 0 : w.n > 8 ? 8 : w.n;
@@ -150,15 +149,15 @@ __global__ __launch_bounds__(A8_THREADS) void k_act8_unpack(const int8_t* codes,
 int a8_check(int dtype, int64_t rows, int cols, int64_t rs) {
   if (dtype != VIL_DTYPE_F32 && dtype != VIL_DTYPE_BF16 && dtype != VIL_DTYPE_F16) return VIL_E_DTYPE;
   if (rows < 0 || cols < 0 || (rows > 1 && rs < cols)) return VIL_E_SHAPE;
-  // (a block of 32, filled or not, is four lanes: 2^31 workgroups of 512 lanes hold more than 2^37 values)
-  if (cols > 0 && rows > ((int64_t)1 << 37) / cols) return VIL_E_SHAPE;
+  // a block of 32, filled or not, is four lanes, and a launch takes fewer than 2^32: 2^24 - 1 workgroups of A8_CHUNKS * A8_THREADS / 4 blocks
+  if (cols > 0 && rows > ((int64_t)(1 << 24) - 1) * (A8_CHUNKS * A8_THREADS / 4) / ((cols - 1) / A8_BLOCK + 1)) return VIL_E_SHAPE;
   return VIL_OK;
 }
 // FLAT: rows of whole blocks without gaps, at addresses that the widest access fits; `rows` is then the number of values
 struct A8Shape { int64_t rows; int cols, nb; bool flat; unsigned grid; };
 A8Shape a8_shape(int64_t rows, int cols, int64_t rs, uintptr_t addresses) {
   A8Shape w;
-  w.nb = (cols + A8_BLOCK - 1) / A8_BLOCK;
+  w.nb = (cols - 1) / A8_BLOCK + 1;
   w.cols = cols;
   w.flat = cols % A8_BLOCK == 0 && (rs == cols || rows == 1) && addresses % 16 == 0;
   const int64_t lanes = rows * w.nb * 4, per = A8_THREADS * A8_CHUNKS;
