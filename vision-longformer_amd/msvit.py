@@ -135,7 +135,8 @@ class _TableGather(torch.autograd.Function):
 
 
 class Mlp(nn.Module):
-    """act8: keep the block's input and hidden pre-activation in 8 bits for the backward pass (act8.vil_mlp_act8: 29 % of the bytes)"""
+    """act8: keep the block's input and hidden pre-activation in 8 bits for the backward pass (act8.vil_mlp_act8: 29 % of the bytes);
+    an exact GELU without dropout, other blocks run as without act8"""
 
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0., act8=False):
         super().__init__()
@@ -147,8 +148,10 @@ class Mlp(nn.Module):
 
     def forward(self, x):
         if isinstance(self.act, nn.GELU) and self.act.approximate == "none" and (self.drop.p == 0.0 or not self.training):
-            if self.act8 and x.is_cuda and torch.is_grad_enabled():
-                return vil_mlp_act8(x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias)
+            args = (x, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias)
+            # (a frozen block of a frozen input keeps nothing for a backward pass: nothing is packed)
+            if self.act8 and x.is_cuda and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+                return vil_mlp_act8(*args)
             # fc1 with the GELU in its epilogue where the weights-in-registers GEMM serves the shape (csrc/vil_gemm_skinny.hip),
             # fc2 with the GELU in front of it as one autograd node: its input gradient is ONE launch (dgrad GEMM with the
             # erf-GELU backward in the epilogue, csrc/vil_gemm_fused.hip)
