@@ -19,3 +19,12 @@ def test_products_with_an_epilogue_hold_no_scratch(kernel, waves):
     assert len(res) == 3, sorted(res)                            # plain, GELU, GELU in its 8-bit form
     for k, v in res.items():
         assert v["scratch"] == 0 and v["occupancy"] >= waves, (k, v)
+
+
+def test_build_takes_the_arguments_that_it_took():
+    """build(), build(True) and build(force=...) are calls that callers have; nothing is compiled here"""
+    import inspect
+    sys.path.insert(0, ROOT)
+    import __graft_entry__ as g
+    for args, kw in (((), {}), ((True,), {}), ((), dict(force=True)), ((), dict(force=False))):
+        inspect.signature(g.build).bind(*args, **kw)
