@@ -24,7 +24,7 @@ Extra objects on the same line:
                 tagged with its problem shape); achieved = ALGORITHMIC bytes of the launch /
                 its average duration.  `traffic` = PMC HBM bytes per launch of
                 that kernel at that shape, collected inside the real step (tools/pmc_step.sh ->
-                profiles/r06_pmc_traffic.json) and attached ONLY when the kernel sources'
+                profiles/step_pmc_traffic.json) and attached ONLY when the kernel sources'
                 fingerprint matches the build that is running.
   roofline_by_shape   the same for fwd / dQ / dK+dV / delta at every hot-path shape of the
                 workload, plus `backward_unit`: SURVEY 8(d)'s whole-backward definition
@@ -375,7 +375,7 @@ def pmc_traffic(config, B, kernel, label):
     from vision_longformer_amd import _lib
     import glob
     fp = _lib.source_fingerprint()
-    for path in sorted(glob.glob(os.path.join(ROOT, "profiles", "r*_pmc_traffic.json")), reverse=True):   # newest round first
+    for path in sorted(glob.glob(os.path.join(ROOT, "profiles", "*_pmc_traffic.json")), reverse=True):    # (step_: the current sources')
         try:
             pm = json.load(open(path))
             if pm.get("source_fingerprint") != fp:
