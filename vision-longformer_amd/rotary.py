@@ -304,6 +304,10 @@ class GridTurn:
         self.sections, self.base, self.layout = (pairs - pairs // 2, pairs // 2), base, layout
         self._made = {}
 
+    def __getstate__(self):
+        # a copy or a pickle makes its own: loaded onto another device, these would be there under this one's name
+        return {**self.__dict__, "_made": {}}
+
     def of(self, nx, ny, nglo, device):
         key = (int(nx), int(ny), int(nglo), device)
         made = self._made.get(key)
