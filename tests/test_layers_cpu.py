@@ -28,3 +28,34 @@ def test_a_grid_s_positions_do_not_travel(how):
     assert (again.sections, again.base, again.layout) == (turn.sections, turn.base, turn.layout)
     for k, v in again.of(3, 2, 1, torch.device("cpu")).items():
         assert torch.equal(v, made[k]) if torch.is_tensor(v) else v == made[k]
+
+
+def before_the_options(m):
+    """the module as a pickle from before the options holds it"""
+    state = {k: v for k, v in m.__dict__.items() if k not in ("q_norm", "k_norm", "turn", "act8")}
+    old = type(m).__new__(type(m))
+    old.__setstate__(state)
+    return old
+
+
+def test_layers_pickled_before_the_options_run():
+    x = torch.randn(2, 17, 32)
+    for m in (Attention(32, num_heads=2, rpe=True, wx=4, wy=4, nglo=1), Mlp(32, 64), Long2DSCSelfAttention(32, num_heads=2, w=4, sharew=True)):
+        old = before_the_options(m)
+        assert [n for n, _ in old.named_modules()] == [n for n, _ in m.named_modules()]
+        if isinstance(m, Long2DSCSelfAttention):
+            assert old.q_norm is None and old.k_norm is None and old.turn is None        # (runs on the device alone)
+        else:
+            args = (x, 4, 4) if isinstance(m, Attention) else (x,)
+            assert torch.equal(old(*args), m(*args))
+
+
+def test_layers_with_the_options_keep_them_through_a_pickle():
+    for m in (Attention(32, num_heads=2, wx=4, wy=4, qk_norm=True, rotary=True),
+              Long2DSCSelfAttention(32, num_heads=2, w=4, sharew=True, qk_norm=True, rotary=True), Mlp(32, 64, act8=True)):
+        for again in (copy.deepcopy(m), through_a_pickle(m)):
+            assert list(again.state_dict()) == list(m.state_dict())
+            if isinstance(m, Mlp):
+                assert again.act8
+            else:
+                assert torch.equal(again.q_norm.weight, m.q_norm.weight) and again.turn.sections == m.turn.sections

@@ -23,7 +23,7 @@ from torch import nn
 
 from .ops import (vil_local_attention, vil_full_attention, vil_full_attention_qkv, vil_global_attention, vil_rotary_attention_qkv,
                   FULL_MAX_G)
-from .rotary import GridTurn, HeadNorm
+from .rotary import GridTurn, HeadNorm, QKOptions
 from .linear import VilLinear, vil_linear, vil_linear_pair
 
 
@@ -47,7 +47,7 @@ def build_relative_position_index(w):
     return torch.cat(blocks, dim=1)
 
 
-class Long2DSCSelfAttention(nn.Module):
+class Long2DSCSelfAttention(QKOptions, nn.Module):
     def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0., proj_drop=0., w=7, d=1,
                  autoregressive=False, sharew=False, nglo=1, only_glo=False, exact=0, autograd=False, rpe=False,
                  mode=0, qk_norm=False, rotary=False):

@@ -19,7 +19,7 @@ from torch import nn
 
 from .longformer2d import Long2DSCSelfAttention, _trunc_normal_
 from .ops import vil_dense_attention, vil_rotary_attention_qkv, dense_family_supported, FULL_MAX_G
-from .rotary import GridTurn, HeadNorm
+from .rotary import GridTurn, HeadNorm, QKOptions
 from .act8 import vil_mlp_act8
 from .layernorm import (VilLayerNorm, res_layernorm, res_layernorm_ok, tokens_layernorm, tokens_layernorm_ok,
                         pass_layernorm, pass_layernorm_ok)
@@ -137,6 +137,7 @@ class _TableGather(torch.autograd.Function):
 class Mlp(nn.Module):
     """act8: keep the block's input and hidden pre-activation in 8 bits for the backward pass (act8.vil_mlp_act8: 29 % of the bytes);
     an exact GELU without dropout, other blocks run as without act8"""
+    act8 = False                                        # (a block that was pickled before it had the option)
 
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0., act8=False):
         super().__init__()
@@ -160,7 +161,7 @@ class Mlp(nn.Module):
         return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
 
 
-class Attention(nn.Module):
+class Attention(QKOptions, nn.Module):
     """Dense multi-head attention with optional relative position bias over an
     (nglo + wx*wy)-token sequence: the `s0` stages (reference msvit.py:37-120)."""
 

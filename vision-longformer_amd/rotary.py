@@ -290,6 +290,16 @@ class HeadNorm(torch.nn.Module):
         self.weight = torch.nn.Parameter(torch.ones(head_dim))
 
 
+class QKOptions:
+    """Of layers with q_norm, k_norm and turn: one that was pickled before it had them has none."""
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ("q_norm", "k_norm", "turn"):
+            if not hasattr(self, name):
+                setattr(self, name, None)
+
+
 class GridTurn:
     """The rotation of a layer on an nx x ny token grid behind nglo global tokens: half of a head's pairs turn with the row,
     half with the column (the rows take the odd one).  `of(nx, ny, nglo, device)` gives vil_rotary_attention_qkv's positions,
