@@ -91,3 +91,29 @@ def test_rows_beside_a_sliced_projection_are_left_alone():
     out = ops.vil_rotary_attention_qkv(**{**a, "qkv": qkv}, backend="mfma")
     g, = torch.autograd.grad(out, qkv, torch.ones_like(out))
     assert torch.equal(wide, keep) and g.shape == qkv.shape and bool(torch.isfinite(g).all())
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp32"])
+@pytest.mark.parametrize("nx,ny,nglo,M", [(6, 9, 1, 32), (9, 6, 0, 48), (3, 14, 2, 64), (1, 7, 1, 32), (11, 10, 0, 64)])
+def test_dense_attention_on_a_grid_that_is_not_square(nx, ny, nglo, M, t):
+    """w None: all tokens attend to all, in the dense family (16 bits, 64 channels) and as one chunk of side max(nx, ny).  Bounds of the
+    attention kernels' own tests, as in test_gpu_4_block.py."""
+    from test_gpu_4_block import attention64
+    H, t = 2, TYPES[t]
+    a = args(None, t, nx=nx, ny=ny, nglo=nglo, H=H, M=M)
+    for n in ("bias_table", "g2l_bias", "g2g_bias"):
+        a[n] = None
+    turn = {k: a[k] for k in ("positions", "inv_freq", "sections")}
+    leaves = [a[n].requires_grad_() for n in ("qkv", "q_weight", "k_weight")]
+    dout = rnd(2, nglo + nx * ny, H * M, seed=3, t=t)
+    out = ops.vil_rotary_attention_qkv(**a)
+    got = torch.autograd.grad(out, leaves, dout)
+    d = [v.detach().double().cpu().requires_grad_() for v in leaves]
+    ref = attention64(d[0], H, d[1], d[2], turn, M ** -0.5)
+    want = torch.autograd.grad(ref, d, dout.double().cpu())
+    low = t != torch.float32
+    err = (out.detach().double().cpu() - ref.detach()).abs()
+    assert bool((err <= (2e-2 + 5e-2 * ref.abs() if low else 2e-5 + 1e-4 * ref.abs())).all()), float(err.max())
+    for x, y in zip(got, want):
+        err, s = (x.double().cpu() - y).abs(), float(y.square().mean().sqrt())
+        assert bool((err <= (0.06 * s + 5e-2 * y.abs() if low else 1e-4 * max(s, 1) + 1e-3 * y.abs())).all()), float(err.max() / s)
