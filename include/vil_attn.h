@@ -486,7 +486,7 @@ int vil_qk_rope_bwd(const VilRopeDesc* d, const void* gq, const void* gk, const 
  * vil_gelu_act8_fwd: a = gelu(h) (exact form) and the packed h.  vil_gelu_act8_bwd: with v = the values the packed h stands
  * for, dh = da * gelu'(v) and, unless a is NULL, a = gelu(v): the input of the next projection's weight gradient, so that
  * neither h nor gelu(h) need be kept in 16 bits (the reference keeps both: Mlp, src/models/msvit.py:17-34).
- * a, dh and y are contiguous. */
+ * a, dh and y are contiguous.  At most 2^31 - 128 blocks (rows * ceil(cols / 32)): VIL_E_SHAPE beyond. */
 int vil_act8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t x_row_stride, void* codes, void* scales, void* stream);
 int vil_act8_unpack(const void* codes, const void* scales, int64_t rows, int cols, void* y, int dtype, void* stream);
 int vil_gelu_act8_fwd(const void* h, int dtype, int64_t rows, int cols, int64_t h_row_stride, void* a, void* codes, void* scales,

@@ -154,8 +154,8 @@ def _linear(x2, w, b):
 # fc1 with the GELU and the packing in its epilogue, and fc2's input gradient with the GELU's backward on the packed form in its
 # epilogue (csrc/vil_gemm_fused.hip), against the library's product and vil_act8.hip's pass over its output; N = 4 K, device us, fused / separate:
 #   T x K     100352 x 96   100352 x 192   25088 x 384   25088 x 768   25088 x 1024   2048 x 192    1024 x 384    512 x 192
-#   forward      50 / 55       108 / 150       63 / 71      185 / 191      322 / 271    8.5 / 9.6    9.9 / 11.1    8.0 / 8.0
-#   backward     56 / 76       137 / 187       76 / 92      240 / 227      378 / 327     10 / 11     13.2 / 13.0   9.8 / 8.1
+#   forward      51 / 55       104 / 149       67 / 72      182 / 192      320 / 269    8.5 / 9.6    9.9 / 11.1    8.0 / 8.2
+#   backward     55 / 74       138 / 186       76 / 90      236 / 232      382 / 328    9.8 / 11.5   12.4 / 13.1   9.2 / 8.7
 # A longer K makes the product the larger part, and the library's is the faster one; few tokens are few tiles.
 _FUSE_MIN_T = 1024
 _FUSE_FWD_MAX_K, _FUSE_BWD_MAX_K = 768, 384

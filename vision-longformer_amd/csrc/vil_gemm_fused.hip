@@ -104,8 +104,8 @@ __device__ __forceinline__ void gf_store1(void* base, unsigned byte_off, unsigne
 // All of a tile's codes (16 registers) and scales (one: lane i has row i's pair, handed to its four lanes in the epilogue) are
 // requested in front of the K loop and claimed before the first store: half the bytes of h leave no reason for two batches.
 // 127 registers, no scratch.  128 is the limit: at 136 (a bound of 3 waves a SIMD) one workgroup less fits a CU, 103 us for 78 at
-// 25088 x 384 -> 1536.  Against the separate product and pass (T x K -> N, us): 100352 x 96 -> 384 55 / 76, 100352 x 192 -> 768
-// 138 / 187, 25088 x 384 -> 1536 78 / 92; K = 768 is slower (242 / 227) and left to the library.
+// 25088 x 384 -> 1536.  Against the separate product and pass (T x K -> N, us): 100352 x 96 -> 384 55 / 74, 100352 x 192 -> 768
+// 138 / 186, 25088 x 384 -> 1536 76 / 90; K = 768 is slower (25088: 236 / 232) and left to the library.
 template <bool DGELU, bool PACK = false>
 __global__ __launch_bounds__(GF_THREADS, 4) void k_dgrad_dgelu(DgParams p) {
   typedef __bf16 T_;
@@ -349,7 +349,7 @@ __device__ __forceinline__ float gelu_fwd(float x) {
 
 // GELU = false: the plain forward h = x W^T + b (vil_gemm_tile_bf16 op 0): one output.  PACK: the rounded h is packed to 8 bits in
 // place of its store; the maximum of a block of 32 features is that of a row's four lanes, 16 apart.  Against the separate product and
-// pass (us): 100352 x 96 -> 384 50 / 55, 100352 x 192 -> 768 108 / 150, 25088 x 384 -> 1536 63 / 71.
+// pass (us): 100352 x 96 -> 384 51 / 55, 100352 x 192 -> 768 104 / 149, 25088 x 384 -> 1536 67 / 72.
 template <bool GELU, bool PACK = false>
 __global__ __launch_bounds__(GF_THREADS, 3) void k_fwd_gelu(FgParams p) {
   typedef __bf16 T_;

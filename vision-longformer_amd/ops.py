@@ -604,7 +604,8 @@ def vil_rotary_attention_qkv(qkv, bias_table, g2l_bias, g2g_bias, *, nx, ny, ngl
                              sections=None, layout="half", norm=False, eps=1e-6):
     """vil_full_attention_qkv (w = the window) or vil_dense_attention (w = None) of a packed (B, N, 3C) projection whose q and k
     first pass vil_rope (norm=False) or vil_qk_norm_rope (norm=True; the weights may be None): one autograd node, v read in
-    place (with w, from rows that follow each other; from others it is copied).  Arguments as those functions'; positions (N, axes) or (B, N, axes) cover the nglo global tokens, which come first."""
+    place (outside the dense family from rows that follow each other; from others it is copied).  Arguments as those functions';
+    positions (N, axes) or (B, N, axes) cover the nglo global tokens, which come first."""
     if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads):
         raise ValueError(f"vil_rotary_attention_qkv: a packed projection of {num_heads} heads; got {tuple(qkv.shape)}")
     if qkv.shape[1] != nglo + nx * ny:
