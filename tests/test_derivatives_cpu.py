@@ -11,7 +11,12 @@ from vision_longformer_amd import _lib, act8, rotary
 def launched(monkeypatch):
     """names of the entry points that a test reaches"""
     names = []
-    monkeypatch.setattr(_lib, "launch", lambda index, fn, *args: names.append(fn.__name__))
+
+    def launch(index, fn, *args):
+        assert torch._C._get_tracing_state() is None            # (where the launch itself would refuse)
+        names.append(fn.__name__)
+
+    monkeypatch.setattr(_lib, "launch", launch)
     monkeypatch.setattr(rotary, "_check", lambda *a: None)
     monkeypatch.setattr(act8, "_check", lambda *a: None)
     monkeypatch.setattr(act8, "_check_packed", lambda *a: None)
@@ -106,7 +111,29 @@ def test_calls_without_a_node_are_not_traced(fn, monkeypatch):
         torch.jit.trace(fn, (torch.randn(4, 64),), check_trace=False)
 
 
-def test_a_traced_8_bit_gelu_launches(launched):
-    traced = torch.jit.trace(act8.vil_gelu_act8, (torch.randn(4, 64),), check_trace=False)
+@pytest.mark.parametrize("op", ["gelu", "mlp"])
+def test_a_traced_8_bit_node_launches(op, launched):
+    ws = [torch.randn(s) for s in ((128, 64), (128,), (64, 128), (64,))]
+    traced = torch.jit.trace(act8.vil_gelu_act8 if op == "gelu" else lambda x: act8.vil_mlp_act8(x, *ws), (torch.randn(4, 64),), check_trace=False)
     n = len(launched)
-    assert traced(torch.randn(4, 64)).shape == (4, 64) and launched[n:] == ["vil_gelu_act8_fwd"]
+    assert traced(torch.randn(4, 64)).shape == (4, 64) and "vil_gelu_act8_fwd" in launched[n:]
+
+
+def test_a_failing_call_leaves_the_trace_on(monkeypatch):
+    """(the node turns tracing off while it runs)"""
+    class Node(torch.autograd.Function):
+        @staticmethod
+        @_lib.untraced
+        def forward(ctx, x):
+            assert torch._C._get_tracing_state() is None and type(x.shape[0]) is int
+            raise KeyError("no")
+
+    def fn(x):
+        on = torch._C._get_tracing_state()
+        assert on is not None
+        with pytest.raises(KeyError):
+            Node.apply(x)
+        assert torch._C._get_tracing_state() is not None
+        return x + 1
+
+    torch.jit.trace(fn, (torch.ones(3),), check_trace=False)

@@ -277,7 +277,7 @@ def check(code):
 def launch(index, fn, *args):
     """fn(*args, stream) on device `index` and its current stream.  The two torch._C calls are what torch.cuda.current_device() and
     current_stream() end in, without the objects around them (8 of the 25 microseconds that a small call took)."""
-    if torch._C._get_tracing_state() is not None:        # (off inside an autograd node, which a trace records and runs again)
+    if torch._C._get_tracing_state() is not None:        # (`untraced` turns it off in a node, which a trace records and runs again)
         raise RuntimeError(f"{fn.__name__}: a trace would record the outputs' allocation and no launch")
     if torch._C._cuda_getDevice() == index:
         code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -286,6 +286,22 @@ def launch(index, fn, *args):
             code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if code != 0:
         check(code)
+
+
+def untraced(forward):
+    """For a node's forward: what it does belongs to the node also while a trace records that, so no launch is refused in it and
+    sizes are numbers."""
+    @functools.wraps(forward)
+    def run(ctx, *args):
+        state = torch._C._get_tracing_state()
+        if state is None:
+            return forward(ctx, *args)
+        torch._C._set_tracing_state(None)
+        try:
+            return forward(ctx, *args)
+        finally:
+            torch._C._set_tracing_state(state)
+    return run
 
 
 def first_derivative_only(backward):

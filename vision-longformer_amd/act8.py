@@ -127,6 +127,7 @@ def vil_gelu_act8_bwd(packed, da, want_act=True):
 
 class _GeluAct8Fn(torch.autograd.Function):
     @staticmethod
+    @_lib.untraced
     def forward(ctx, h):
         a, packed = vil_gelu_act8_fwd(h)
         ctx.save_for_backward(packed.codes, packed.scales)
@@ -211,6 +212,7 @@ def _weight_grad(dy2, x2, w, want_b):
 class _MlpAct8Fn(torch.autograd.Function):
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
+    @_lib.untraced
     def forward(ctx, x, w1, b1, w2, b2):
         x2 = _rows(x)
         fused = _fused_fwd(x2, w1, b1)

@@ -534,6 +534,7 @@ class _VilRotaryAttention(torch.autograd.Function):
     the rotation's backward pass writes straight from the attention's."""
 
     @staticmethod
+    @_lib.untraced
     def forward(ctx, qkv, table, g2l, g2g, wq, wk, positions, inv_freq, cfg, turn, backend):
         from . import rotary
         B, N, C3 = qkv.shape

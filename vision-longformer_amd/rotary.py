@@ -191,6 +191,7 @@ def _bwd(plan, desc, gq, gk, q, k, wq, wk, positions, inv_freq, dq, dk, need_wq,
 
 class _QKRope(torch.autograd.Function):
     @staticmethod
+    @_lib.untraced
     def forward(ctx, q, k, wq, wk, positions, inv_freq, plan):
         """plan: a _Plan of tensors that _inputs has seen, or _inputs' name and options"""
         if not isinstance(plan, _Plan):
