@@ -274,10 +274,13 @@ def check(code):
         raise VilAttnError(code, lib().vil_attn_strerror(code).decode())
 
 
+_trace = torch._C._get_tracing_state         # (None: no trace)
+
+
 def launch(index, fn, *args):
     """fn(*args, stream) on device `index` and its current stream.  The two torch._C calls are what torch.cuda.current_device() and
     current_stream() end in, without the objects around them (8 of the 25 microseconds that a small call took)."""
-    if torch._C._get_tracing_state() is not None:        # (`untraced` turns it off in a node, which a trace records and runs again)
+    if _trace() is not None:        # (`untraced` turns it off in a node, which a trace records and runs again)
         raise RuntimeError(f"{fn.__name__}: a trace would record the outputs' allocation and no launch")
     if torch._C._cuda_getDevice() == index:
         code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -293,7 +296,7 @@ def untraced(forward):
     sizes are numbers."""
     @functools.wraps(forward)
     def run(ctx, *args):
-        state = torch._C._get_tracing_state()
+        state = _trace()
         if state is None:
             return forward(ctx, *args)
         torch._C._set_tracing_state(None)

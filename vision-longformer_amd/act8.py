@@ -40,8 +40,8 @@ def _check(x, name):
         raise TypeError(f"{name} supports float32 / bfloat16 / float16; got {x.dtype}")
     if x.dim() < 1:
         raise ValueError(f"{name}: a tensor with at least one axis")
-    cols = x.shape[-1]
-    if cols >= 2 ** 31 or (cols and x.numel() // cols * -(-cols // BLOCK) > _MAX_BLOCKS):
+    n, cols = x.numel(), x.shape[-1]
+    if cols >= 2 ** 31 or (n > _MAX_BLOCKS and n // cols * -(-cols // BLOCK) > _MAX_BLOCKS):
         raise ValueError(f"{name}: {tuple(x.shape)} is too large (2^31 blocks of {BLOCK} channels, filled or not)")
     if not x.is_cuda:
         raise RuntimeError(f"{name} needs device tensors: the product path is the HIP kernels (libvilattn.so); there is no CPU "

@@ -246,7 +246,7 @@ def _inputs(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps
 
 
 def _apply(name, q, k, wq, wk, positions, inv_freq, sections, layout, norm, eps):
-    if forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None:
+    if forward_ad._current_level >= 0 or _lib._trace() is not None:
         # a tangent, which only the node refuses; a trace, which records the node and not the launch, and whose sizes are no
         # numbers outside it
         yq, yk = _QKRope.apply(q, k, wq, wk, positions, inv_freq, (name, sections, layout, norm, eps))
